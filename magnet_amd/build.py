@@ -14,6 +14,7 @@ from __future__ import annotations
 import concurrent.futures as cf
 import glob
 import os
+import re
 import subprocess
 import sys
 
@@ -21,7 +22,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libmagnet_hip.so")
 ARCH = "gfx950"
-FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wno-unused-result", *os.environ.get("MAGNET_BUILD_DEFS", "").split()]   # MAGNET_BUILD_DEFS: extra -D... of an experiment build
+# (-packed-fp32-ops: some forms of the packed fp32 instructions that -O3 makes of ordinary float code have given wrong results on these cards)
+FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-result", *os.environ.get("MAGNET_BUILD_DEFS", "").split()]   # MAGNET_BUILD_DEFS: extra -D... of an experiment build
 # per-source additions: the lane-per-node read-out is one fully unrolled block; below the default pragma-unroll threshold
 # hipcc unrolls it partially, indexes the row registers dynamically and puts them in scratch
 # mpnn_edge_rows.hip: hipcc's SLP vectoriser pairs the epilogue's per-value fma into v_pk_fma_f32 and pays two v_mov per pair to line the
@@ -52,10 +54,20 @@ def needs_build(lib: str = LIB) -> bool:
 DEV_LIB = os.path.join(CSRC, "libmagnet_hip_dev.so")
 
 
+def _included(src: str, seen: set | None = None) -> set:
+    """a source and the headers of this folder that it includes, directly or not"""
+    seen = set() if seen is None else seen
+    seen.add(src)
+    for name in re.findall(r'^\s*#include\s+"([^"]+)"', open(src).read(), re.M):
+        p = os.path.join(CSRC, name)
+        if p not in seen and os.path.exists(p):
+            _included(p, seen)
+    return seen
+
+
 def _compile(src: str, dev: bool = False) -> str:
     obj = os.path.splitext(src)[0] + (".dev.o" if dev else ".o")
-    hdr = max(os.path.getmtime(p) for p in glob.glob(os.path.join(CSRC, "*.cuh")))
-    if os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(src), hdr):
+    if os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(p) for p in _included(src)):
         return obj
     cmd = ["hipcc", *FLAGS, *(["-DMAGNET_DEV_VARIANTS"] if dev else []), *EXTRA_FLAGS.get(os.path.basename(src), []), "-c", src,
            "-o", obj]
