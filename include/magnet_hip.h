@@ -544,6 +544,43 @@ int magnet_mpnn_edge_bwd_w_flags_f32(const float* A, const float* Bm, const floa
                                      const float* b2, float* dp, float* dA, float* partials, float* dW2, float* db2, int accumulate,
                                      float* workspace, const float* amax_in, int n_amax_in, int flags, void* stream);
 
+/* ---- 8-bit activation tape (csrc/tape8.cuh) and what reads it.  No reference counterpart: torch autograd keeps the activations of
+ *      models/backbones/mlp.py:9-28 in fp32.  A tape of M rows of W values: codes [M][32 ceil(W / 32)] (16-byte aligned) and one byte per
+ *      block of 32 columns, bytes [M][ceil(W / 32)]; value = code 2^(byte - 127), byte 0 = zeros, 255 = NaN (the block held a value that is
+ *      not finite).  kind 0 (signed): code = round(x / step) in [-127, 127]; kind 1 (behind a ReLU): 0 where x <= 0, else in [1, 255].
+ *      dtype: 0 = fp32, 1 = bf16, 2 = fp16.  Row strides (ld*) count elements. ---- */
+int magnet_tape8_pack(const void* x, int dtype, long ldx, long M, int W, int kind, void* codes, void* bytes, void* stream);
+int magnet_tape8_unpack(const void* codes, const void* bytes, long M, int W, int kind, void* y, int dtype, long ldy, void* stream);
+/* A Linear y = x W^T + b walked back from the tape of its input (torch autograd of nn.Linear and its activation, models/backbones/mlp.py:9-28,
+ * models/mpnn.py:15-24,81-90), any N, K >= 1: with v the tape's values and x = act(v)
+ *   dx [M][K] = act'(v) (dz W),  dW [N][K] (+)= dz^T x,  db [N] (+)= column sums of dz       (dx, db may be NULL)
+ * act: MAGNET_ACT_NONE (signed tape of x), _RELU (relu tape of x: act' = x > 0), _SWISH (signed tape of Swish's argument).  dx must not
+ * overlap dz.  M = 0 zeroes dW / db (accumulate == 0).  workspace: magnet_tape8_linear_bwd_workspace(M, N, K) floats. */
+int magnet_tape8_linear_bwd_workspace(long M, int N, int K, long* floats);
+int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void* codes, const void* bytes, const float* w, long ldw, long M, int N, int K,
+                                int act, float* dx, long lddx, float* dW, long lddw, float* db, int accumulate, float* workspace,
+                                void* stream);
+/* The end of a residual block and the beginning of the next one (the residual and LayerNorm around InteractionNetwork's MLPs,
+ * models/magnet_gnn.py:38-42,79-90, in their general form), rows of W <= 4096 values, dtype 0 or 1 for x, f, gate, y, h:
+ *   t = post(f),  y = x + scale * gate * t,  h = pre(y)
+ * post / pre: (v - mean) / sqrt(var + eps) (layer != 0) or v / sqrt(mean v^2 + eps), times gain, plus bias (NULL: none); gain NULL: no such
+ * norm (t = f; h is not written).  scale_v [W] or NULL: the number `scale`.  gate [G][W] or NULL, M % G == 0: row r takes gate row
+ * r / (M / G).  Statistics and sums are fp32; y and h are rounded to dtype once, h is formed from y before it is rounded.
+ * post_codes != NULL: the normalised rows (f itself without a post norm) go onto signed tapes, 1 / sqrt(..) into *_rstd [M]. */
+int magnet_norm_join(const void* x, long ldx, const void* f, long ldf, int dtype, long M, int W, int layer, float eps, const float* post_g,
+                     const float* post_b, const float* pre_g, const float* pre_b, const void* gate, long ldg, long G, const float* scale_v,
+                     float scale, void* y, void* h, void* post_codes, void* post_bytes, float* post_rstd, void* pre_codes, void* pre_bytes,
+                     float* pre_rstd, void* stream);
+/* Its backward from gy = d y, gh = d h (pre norm only) and the tapes: dx, df [M][W], dgate [G][W] (dtype), d_scale / d_post_g / d_post_b /
+ * d_pre_g / d_pre_b [W] (fp32, written; NULL: not wanted).  M >= 1.  workspace: magnet_norm_join_bwd_workspace(M, W, G or 0) floats.  The sums
+ * over rows are added in a fixed order. */
+int magnet_norm_join_bwd_workspace(long M, int W, long G, long* floats);
+int magnet_norm_join_bwd(const void* gy, long ldgy, const void* gh, long ldgh, int dtype, long M, int W, int layer, const float* post_g,
+                         const float* post_b, const float* pre_g, const float* pre_b, const void* gate, long ldg, long G, const float* scale_v,
+                         float scale, const void* post_codes, const void* post_bytes, const float* post_rstd, const void* pre_codes,
+                         const void* pre_bytes, const float* pre_rstd, void* dx, void* df, void* dgate, float* d_scale, float* d_post_g,
+                         float* d_post_b, float* d_pre_g, float* d_pre_b, float* workspace, void* stream);
+
 /* Weight packing on the device (magnet_amd/packing.py: the same layouts as torch index shuffles; no reference counterpart - the
  * reference hands its nn.Linear weights to cuBLAS as they are).  Padded position (r, c) of the [np x kp] matrix takes
  * w[r' stride_r + c' stride_c] with r' = row_src ? row_src[r] : r (r < n) and c' = col_src ? col_src[c] : c (c < k); -1 / out of

@@ -1,0 +1,455 @@
+// A residual block's end and the next block's beginning in one pass over the rows:
+//     t = post(f)      y = x + scale * gate * t      h = pre(y)
+// post / pre: LayerNorm (v - mean) / sqrt(var + eps) * gain + bias, RMS norm v / sqrt(mean v^2 + eps) * gain, or absent (t = f, no h); scale:
+// a number or one per column; gate: one row for every M / G consecutive rows (G = M: one for every element), or absent.  For training
+// the rows of both norms before gain and bias go onto an 8-bit tape (tape8.cuh) with the factors 1 / sqrt(..): the normalised row is
+// what the backward pass needs, and its values are of the order of one whatever f was (a tape of f itself would lose a small variation on a
+// large mean).
+//
+// Backward, from gy = d y and gh = d h, v^ the taped rows, r their factors:
+//     u = gh pre_gain      D = gy + r_pre (u - [mean u] - y^ mean(u y^))                     dx = D
+//     v = scale gate D     u = v post_gain      df = r_post (u - [mean u] - f^ mean(u f^))   (no post: df = v)
+//     d gate = scale t D summed over its rows; d scale = sum gate t D; d post_gain = sum v f^; d post_bias = sum v;
+//     d pre_gain = sum gh y^; d pre_bias = sum gh                                            ([mean u]: LayerNorm only)
+// All four sums over rows are linear in  S1 = sum gate D f^,  S0 = sum gate D,  P1 = sum gh y^,  P0 = sum gh  - four sums per column.
+//
+// Both are bound by HBM: every array is read or written once.  A row belongs to a team of 16 to 256 lanes, four neighbouring columns per
+// lane and slot, and stays in registers from its load to its last use; statistics are lane exchanges (through LDS for a team of four
+// waves), fp32, the variance around the mean.  Gradients of parameters: a lane adds its columns over the rows that its team walks, teams
+// and workgroups are added in their order (the same bits every time).
+#include "common.cuh"
+#include "tape8.cuh"
+
+struct NjArgs {
+    const void *x, *f, *gate;            // rows of x, f (forward) or gy, gh (backward: x = gy, f = gh)
+    const float *scale_v, *post_g, *post_b, *pre_g, *pre_b;
+    void *y, *h;                         // outputs: y, h (forward) or df, dx (backward: y = dx, h = df)
+    unsigned char *post_c, *post_e, *pre_c, *pre_e;     // tape: codes and bytes of the normalised rows
+    float *post_r, *pre_r;               // [M] factors
+    void* dgate;
+    float* part;                         // backward: [workgroups][4][W] sums S1, S0, P1, P0
+    long M, ldx, ldf, ldg, ldy, ldh;
+    long rows_per_gate;                  // M / G (M without a gate)
+    long groups;                         // backward: G, 1 without a gate
+    int W, vec, layer, has_post, has_pre, has_gate, tape, per_group, own_group, need_sums;
+    float scale, eps;
+};
+
+// sum over a team of TL lanes (a team of 256: the whole workgroup, through LDS)
+template <int TL>
+__device__ __forceinline__ float nj_sum(float v, float* red) {
+    constexpr int L = TL < 64 ? TL : 64;
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) v += __shfl_xor(v, o);
+    if (TL > 64) {
+        __syncthreads();
+        if (!(threadIdx.x & 63)) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+    return v;
+}
+__device__ __forceinline__ float nj_hsum(const t8_f4& v) { return (v[0] + v[1]) + (v[2] + v[3]); }
+__device__ __forceinline__ float nj_dot(const t8_f4& a, const t8_f4& b) { return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]); }
+
+// v -> (v - mean) r or v r in place; returns r.  Columns past the width hold zero before and after.
+template <int TL, int VPT>
+__device__ __forceinline__ float nj_norm(t8_f4 (&v)[VPT], int lane, int W, int layer, float eps, float* red) {
+    const float inv = 1.0f / (float)W;
+    if (layer) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) s += nj_hsum(v[i]);
+        const float mean = nj_sum<TL>(s, red) * inv;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[i][c] = 4 * (i * TL + lane) + c < W ? v[i][c] - mean : 0.f;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) q += nj_dot(v[i], v[i]);
+    const float r = 1.0f / sqrtf(nj_sum<TL>(q, red) * inv + eps);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) v[i] *= r;
+    return r;
+}
+// the normalised row onto the tape
+template <int TL, int VPT>
+__device__ __forceinline__ void nj_tape(const t8_f4 (&v)[VPT], int lane, int W, long row, unsigned char* codes, unsigned char* bytes) {
+    const int blocks = (W + 31) / 32;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int c = 4 * (i * TL + lane);
+        const unsigned byte = t8_byte<T8_SIGNED>(t8_max8(t8_top4<T8_SIGNED>(v[i])));
+        if (c < 32 * blocks) {
+            *reinterpret_cast<unsigned*>(codes + row * (32 * blocks) + c) = t8_code4<T8_SIGNED>(v[i], byte);
+            if (!(lane & 7)) bytes[row * blocks + c / 32] = (unsigned char)byte;
+        }
+    }
+}
+template <int TL, int VPT>
+__device__ __forceinline__ void nj_untape(t8_f4 (&v)[VPT], int lane, int W, long row, const unsigned char* codes, const unsigned char* bytes) {
+    const int blocks = (W + 31) / 32;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int c = 4 * (i * TL + lane);
+        v[i] = c < W ? t8_decode4<T8_SIGNED>(*reinterpret_cast<const unsigned*>(codes + row * (32 * blocks) + c), bytes[row * blocks + c / 32]) : t8_f4{0.f, 0.f, 0.f, 0.f};
+    }
+}
+// a row of parameters (fp32, any alignment of the row's columns past the width reads zero)
+__device__ __forceinline__ t8_f4 nj_par(const float* p, int c, int W, float none) {
+    t8_f4 v = {none, none, none, none};
+    if (!p) return v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i < W ? p[c + i] : 0.f;
+    return v;
+}
+
+__device__ __forceinline__ t8_f4 nj_scale(const NjArgs& a, int c) {
+    return a.scale_v ? nj_par(a.scale_v, c, a.W, 0.f) : t8_f4{a.scale, a.scale, a.scale, a.scale};
+}
+
+template <typename T, int TL, int VPT>
+__global__ void __launch_bounds__(256) k_norm_join(const NjArgs a) {
+    __shared__ float red[4];
+    constexpr int TEAMS = 256 / TL;
+    const int lane = threadIdx.x % TL;
+    const int W = a.W;
+    const T *x = (const T*)a.x, *f = (const T*)a.f, *gate = (const T*)a.gate;
+    T *y = (T*)a.y, *h = (T*)a.h;
+    // (every lane of a wave walks as often as its neighbours: the lane exchanges need them all; rows past the end are clamped and not stored)
+    const long stride = (long)gridDim.x * TEAMS;
+    for (long base = (long)blockIdx.x * TEAMS; base < a.M; base += stride) {
+        const long row = base + threadIdx.x / TL;
+        const bool on = row < a.M;
+        const long r = on ? row : a.M - 1;
+        t8_f4 v[VPT], s[VPT];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = 4 * (i * TL + lane);
+            v[i] = t8_load4(f + r * a.ldf + c, a.vec && c < W, W - c);
+            s[i] = t8_load4(x + r * a.ldx + c, a.vec && c < W, W - c);
+        }
+        if (a.has_post) {
+            const float rs = nj_norm<TL, VPT>(v, lane, W, a.layer, a.eps, red);
+            if (a.tape && on && lane == 0) a.post_r[row] = rs;
+        }
+        if (a.tape && on) nj_tape<TL, VPT>(v, lane, W, row, a.post_c, a.post_e);
+        const long gr = a.has_gate ? r / a.rows_per_gate : 0;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = 4 * (i * TL + lane);
+            t8_f4 t = v[i];
+            if (a.has_post) {
+                t = t * nj_par(a.post_g, c, W, 1.f);
+                if (a.post_b) t += nj_par(a.post_b, c, W, 0.f);
+            }
+            if (a.has_gate) t *= t8_load4(gate + gr * a.ldg + c, a.vec && c < W, W - c);
+            s[i] += nj_scale(a, c) * t;
+            if (on) t8_store4(y + r * a.ldy + c, a.vec && c < W, W - c, s[i]);
+        }
+        if (!a.has_pre) continue;
+        // (the second norm reads y before it is rounded to T)
+        const float rs = nj_norm<TL, VPT>(s, lane, W, a.layer, a.eps, red);
+        if (a.tape && on && lane == 0) a.pre_r[row] = rs;
+        if (a.tape && on) nj_tape<TL, VPT>(s, lane, W, row, a.pre_c, a.pre_e);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = 4 * (i * TL + lane);
+            t8_f4 t = s[i] * nj_par(a.pre_g, c, W, 1.f);
+            if (a.pre_b) t += nj_par(a.pre_b, c, W, 0.f);
+            if (on) t8_store4(h + r * a.ldh + c, a.vec && c < W, W - c, t);
+        }
+    }
+}
+
+// u (times r) without its part along v^ (and, LayerNorm, without its mean): the gradient at a norm's input
+template <int TL, int VPT>
+__device__ __forceinline__ void nj_norm_bwd(t8_f4 (&u)[VPT], const t8_f4 (&vh)[VPT], float r, int lane, int W, int layer, float* red) {
+    const float inv = 1.0f / (float)W;
+    float s = 0.f, p = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) s += nj_hsum(u[i]), p += nj_dot(u[i], vh[i]);
+    p = nj_sum<TL>(p, red) * inv;
+    s = layer ? nj_sum<TL>(s, red) * inv : 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) u[i][c] = 4 * (i * TL + lane) + c < W ? ((u[i][c] - s) - vh[i][c] * p) * r : 0.f;
+}
+
+// Which rows a team walks, and where the sums of a gate row meet:
+//   no gate:          any rows, one set of sums for the launch
+//   G gate rows, few: per_group workgroups for each, their sums stay apart (S1, S0 without the gate) and meet in k_norm_join_gate
+//   many (own_group): a team takes whole gate rows one after the other - up to one for every row - and writes their gradients itself
+template <typename T, int TL, int VPT>
+__global__ void __launch_bounds__(256) k_norm_join_bwd(const NjArgs a) {
+    __shared__ float red[4];
+    __shared__ __attribute__((aligned(16))) float part[TL < 256 ? 256 * 4 : 4];
+    constexpr int TEAMS = 256 / TL;
+    const int lane = threadIdx.x % TL, team = threadIdx.x / TL;
+    const int W = a.W;
+    const T *gy = (const T*)a.x, *gh = (const T*)a.f, *gate = (const T*)a.gate;
+    T *dx = (T*)a.y, *df = (T*)a.h, *dgate = (T*)a.dgate;
+    const long me = (long)blockIdx.x * TEAMS + team;
+    const long g_step = a.own_group ? (long)gridDim.x * TEAMS : a.groups;
+    t8_f4 S1[VPT], S0[VPT], P1[VPT], P0[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) S1[i] = S0[i] = P1[i] = P0[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
+    for (long g = a.own_group ? me : a.per_group ? blockIdx.x / a.per_group : 0; g < a.groups; g += g_step) {
+        const long last = (g + 1) * a.rows_per_gate;
+        long row = g * a.rows_per_gate, step = 1;
+        if (!a.own_group) {
+            row += a.per_group ? (long)(blockIdx.x % a.per_group) * TEAMS + team : me;
+            step = (long)(a.per_group ? a.per_group : gridDim.x) * TEAMS;
+        }
+        t8_f4 T1[VPT], T0[VPT];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) T1[i] = T0[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
+        for (; row < last; row += step) {
+            t8_f4 D[VPT], v[VPT];
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = 4 * (i * TL + lane);
+                D[i] = t8_load4(gy + row * a.ldx + c, a.vec && c < W, W - c);
+            }
+            if (a.has_pre) {
+                t8_f4 u[VPT];
+                nj_untape<TL, VPT>(v, lane, W, row, a.pre_c, a.pre_e);
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) {
+                    const int c = 4 * (i * TL + lane);
+                    u[i] = t8_load4(gh + row * a.ldf + c, a.vec && c < W, W - c);
+                    P0[i] += u[i], P1[i] += u[i] * v[i];
+                    u[i] *= nj_par(a.pre_g, c, W, 1.f);
+                }
+                nj_norm_bwd<TL, VPT>(u, v, a.pre_r[row], lane, W, a.layer, red);
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) D[i] += u[i];
+            }
+            nj_untape<TL, VPT>(v, lane, W, row, a.post_c, a.post_e);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = 4 * (i * TL + lane);
+                t8_store4(dx + row * a.ldy + c, a.vec && c < W, W - c, D[i]);
+                T0[i] += D[i], T1[i] += D[i] * v[i];
+                if (a.has_gate) D[i] *= t8_load4(gate + g * a.ldg + c, a.vec && c < W, W - c);
+                D[i] *= nj_scale(a, c);
+                if (a.has_post) D[i] *= nj_par(a.post_g, c, W, 1.f);
+            }
+            if (a.has_post) nj_norm_bwd<TL, VPT>(D, v, a.post_r[row], lane, W, a.layer, red);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int c = 4 * (i * TL + lane);
+                t8_store4(df + row * a.ldh + c, a.vec && c < W, W - c, D[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            t8_f4 gt = {1.f, 1.f, 1.f, 1.f};
+            if (a.own_group) {
+                const int c = 4 * (i * TL + lane);
+                gt = t8_load4(gate + g * a.ldg + c, a.vec && c < W, W - c);
+                t8_f4 t = T1[i];
+                if (a.has_post) t *= nj_par(a.post_g, c, W, 1.f);
+                if (a.post_b) t += T0[i] * nj_par(a.post_b, c, W, 0.f);
+                t8_store4(dgate + g * W + c, a.vec && c < W, W - c, t * nj_scale(a, c));
+            }
+            S1[i] += gt * T1[i], S0[i] += gt * T0[i];
+        }
+    }
+    if (!a.need_sums) return;
+    // ---- the workgroup's sums: the teams in order
+    float* out = a.part + (size_t)blockIdx.x * 4 * W;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            t8_f4 s = q == 0 ? S1[i] : q == 1 ? S0[i] : q == 2 ? P1[i] : P0[i];
+            const int c = 4 * (i * TL + lane);
+            if (TEAMS > 1) {
+                __syncthreads();
+                *reinterpret_cast<t8_f4*>(&part[4 * threadIdx.x]) = s;
+                __syncthreads();
+                if (team == 0) {
+                    s = *reinterpret_cast<const t8_f4*>(&part[4 * lane]);
+                    for (int t = 1; t < TEAMS; ++t) s += *reinterpret_cast<const t8_f4*>(&part[4 * (t * TL + lane)]);
+                }
+            }
+            if (team == 0)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (c + k < W) out[q * W + c + k] = s[k];
+        }
+}
+
+// sums of a column over n of the workgroups' sets (`first`, first + apart, ..), in order: a workgroup takes 32 columns, eight slices of the sets each; the total in
+// v of slice 0
+__device__ __forceinline__ void nj_fold(const float* part, long first, int n, long apart, int W, int c, float (&v)[4], float (*s)[4][32]) {
+    const int col = threadIdx.x & 31, slice = threadIdx.x >> 5;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = 0.f;
+    if (c < W)
+#pragma unroll 4
+        for (int w = slice; w < n; w += 8) {
+            const float* p = part + (first + w * apart) * 4 * W + c;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] += p[(long)q * W];
+        }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s[slice][q][col] = v[q];
+    __syncthreads();
+    if (slice) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        v[q] = s[0][q][col];
+        for (int k = 1; k < 8; ++k) v[q] += s[k][q][col];
+    }
+}
+// one gate row (blockIdx.y): its gradient, and its workgroups' sums with the gate multiplied in, left in the first one's place
+template <typename T>
+__global__ void __launch_bounds__(256) k_norm_join_gate(const NjArgs a) {
+    __shared__ float s[8][4][32];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), W = a.W;
+    const long g = blockIdx.y;
+    float v[4];
+    nj_fold(a.part, g * a.per_group, a.per_group, 1, W, c, v, s);
+    if (threadIdx.x >= 32 || c >= W) return;
+    const float gt = (float)((const T*)a.gate)[g * a.ldg + c], sc = a.scale_v ? a.scale_v[c] : a.scale;
+    const float t = v[0] * (a.has_post ? a.post_g[c] : 1.f) + (a.post_b ? v[1] * a.post_b[c] : 0.f);
+    ((T*)a.dgate)[g * W + c] = (T)(sc * t);
+    float* p = a.part + g * a.per_group * 4 * W + c;
+    p[0] = gt * v[0], p[W] = gt * v[1], p[2 * W] = v[2], p[3 * W] = v[3];
+}
+// the parameters' gradients from n sets of sums, `apart` sets from one to the next
+__global__ void __launch_bounds__(256) k_norm_join_params(const NjArgs a, int n, int apart, float* d_scale, float* d_post_g, float* d_post_b, float* d_pre_g,
+                                                          float* d_pre_b) {
+    __shared__ float s[8][4][32];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31);
+    float v[4];
+    nj_fold(a.part, 0, n, apart, a.W, c, v, s);
+    if (threadIdx.x >= 32 || c >= a.W) return;
+    const float sc = a.scale_v ? a.scale_v[c] : a.scale;
+    if (d_scale) d_scale[c] = v[0] * (a.has_post ? a.post_g[c] : 1.f) + (a.post_b ? v[1] * a.post_b[c] : 0.f);
+    if (d_post_g) d_post_g[c] = sc * v[0];
+    if (d_post_b) d_post_b[c] = sc * v[1];
+    if (d_pre_g) d_pre_g[c] = v[2];
+    if (d_pre_b) d_pre_b[c] = v[3];
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------- launches
+#define NJ_MAX_W 4096
+static int nj_team(int W) { return W <= 64 ? 16 : W <= 128 ? 32 : W <= 1024 ? 64 : 256; }
+static long nj_grid(long M, int W) {
+    const int teams = 256 / nj_team(W);
+    const long n = (M + teams - 1) / teams;
+    return n < 2048 ? n : 2048;
+}
+// backward: workgroups, and how many of them share a gate row (0: they are not bound to gate rows).  Up to 2048 gate rows get workgroups of
+// their own - a set of sums each, added by a second launch; beyond that a team walks whole gate rows and no sums are kept per row
+static long nj_bwd_grid(long M, int W, long G, int* per_group) {
+    const int teams = 256 / nj_team(W);
+    *per_group = 0;
+    if (G <= 0 || G > 2048 || G == M) {
+        const long n = ((G > 2048 ? G : M) + teams - 1) / teams;
+        return n < 512 ? n : 512;
+    }
+    const long each = (M / G + teams - 1) / teams, n = G < 512 ? 512 / G : 1;
+    *per_group = (int)(each < n ? each : n);
+    return G * *per_group;
+}
+extern "C" int magnet_norm_join_bwd_workspace(long M, int W, long G, long* floats) {
+    int per = 0;
+    if (M < 1 || W < 1 || W > NJ_MAX_W || G < 0 || (G && M % G)) return -2;
+    *floats = nj_bwd_grid(M, W, G, &per) * 4 * W;
+    return 0;
+}
+
+template <typename T>
+static void nj_forward(const NjArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)nj_grid(a.M, a.W));
+    const int W = a.W;
+    if (W <= 64) k_norm_join<T, 16, 1><<<grid, 256, 0, st>>>(a);
+    else if (W <= 128) k_norm_join<T, 32, 1><<<grid, 256, 0, st>>>(a);
+    else if (W <= 256) k_norm_join<T, 64, 1><<<grid, 256, 0, st>>>(a);
+    else if (W <= 512) k_norm_join<T, 64, 2><<<grid, 256, 0, st>>>(a);
+    else if (W <= 1024) k_norm_join<T, 64, 4><<<grid, 256, 0, st>>>(a);
+    else if (W <= 2048) k_norm_join<T, 256, 2><<<grid, 256, 0, st>>>(a);
+    else k_norm_join<T, 256, 4><<<grid, 256, 0, st>>>(a);
+}
+template <typename T>
+static void nj_backward(const NjArgs& a, dim3 grid, hipStream_t st) {
+    const int W = a.W;
+    if (W <= 64) k_norm_join_bwd<T, 16, 1><<<grid, 256, 0, st>>>(a);
+    else if (W <= 128) k_norm_join_bwd<T, 32, 1><<<grid, 256, 0, st>>>(a);
+    else if (W <= 256) k_norm_join_bwd<T, 64, 1><<<grid, 256, 0, st>>>(a);
+    else if (W <= 512) k_norm_join_bwd<T, 64, 2><<<grid, 256, 0, st>>>(a);
+    else if (W <= 1024) k_norm_join_bwd<T, 64, 4><<<grid, 256, 0, st>>>(a);
+    else if (W <= 2048) k_norm_join_bwd<T, 256, 2><<<grid, 256, 0, st>>>(a);
+    else k_norm_join_bwd<T, 256, 4><<<grid, 256, 0, st>>>(a);
+}
+static int nj_vec(int W, size_t size, const void* const* p, const long* ld, int n) {
+    int ok = !(W & 3);
+    for (int i = 0; i < n; ++i)
+        if (p[i]) ok &= !((uintptr_t)p[i] & (4 * size - 1)) && !(ld[i] & 3);
+    return ok;
+}
+
+extern "C" int magnet_norm_join(const void* x, long ldx, const void* f, long ldf, int dtype, long M, int W, int layer, float eps, const float* post_g,
+                                const float* post_b, const float* pre_g, const float* pre_b, const void* gate, long ldg, long G, const float* scale_v,
+                                float scale, void* y, void* h, void* post_codes, void* post_bytes, float* post_rstd, void* pre_codes, void* pre_bytes,
+                                float* pre_rstd, void* stream) {
+    if (M < 0 || W < 1 || W > NJ_MAX_W || ldx < W || ldf < W || (dtype != T8_F32 && dtype != T8_BF16) || (gate && (G < 1 || M % G || ldg < W))) return -2;
+    if (M == 0) return 0;
+    if (!y || (post_b && !post_g) || (pre_b && !pre_g) || (pre_g && !h)) return -2;
+    const int tape = post_codes != nullptr;
+    if (tape && (!post_bytes || (post_g && !post_rstd) || (pre_g && (!pre_codes || !pre_bytes || !pre_rstd)))) return -2;
+    const size_t size = dtype == T8_F32 ? 4 : 2;
+    NjArgs a = {};
+    a.x = x, a.f = f, a.gate = gate, a.scale_v = scale_v, a.post_g = post_g, a.post_b = post_b, a.pre_g = pre_g, a.pre_b = pre_b, a.y = y, a.h = h;
+    a.post_c = (unsigned char*)post_codes, a.post_e = (unsigned char*)post_bytes, a.pre_c = (unsigned char*)pre_codes, a.pre_e = (unsigned char*)pre_bytes;
+    a.post_r = post_rstd, a.pre_r = pre_rstd, a.M = M, a.ldx = ldx, a.ldf = ldf, a.ldg = ldg, a.ldy = W, a.ldh = W;
+    a.rows_per_gate = gate ? M / G : M, a.W = W, a.layer = layer, a.has_post = post_g != nullptr, a.has_pre = pre_g != nullptr, a.has_gate = gate != nullptr;
+    a.tape = tape, a.scale = scale, a.eps = eps;
+    const void* p[] = {x, f, gate, y, h};
+    const long ld[] = {ldx, ldf, ldg, W, W};
+    a.vec = nj_vec(W, size, p, ld, 5);
+    if (dtype == T8_F32) nj_forward<float>(a, (hipStream_t)stream);
+    else nj_forward<__bf16>(a, (hipStream_t)stream);
+    return (int)hipGetLastError();
+}
+
+extern "C" int magnet_norm_join_bwd(const void* gy, long ldgy, const void* gh, long ldgh, int dtype, long M, int W, int layer, const float* post_g,
+                                    const float* post_b, const float* pre_g, const float* pre_b, const void* gate, long ldg, long G, const float* scale_v,
+                                    float scale, const void* post_codes, const void* post_bytes, const float* post_rstd, const void* pre_codes,
+                                    const void* pre_bytes, const float* pre_rstd, void* dx, void* df, void* dgate, float* d_scale, float* d_post_g,
+                                    float* d_post_b, float* d_pre_g, float* d_pre_b, float* workspace, void* stream) {
+    if (M < 1 || W < 1 || W > NJ_MAX_W || ldgy < W || (dtype != T8_F32 && dtype != T8_BF16) || !dx || !df || (gate && (G < 1 || M % G || ldg < W || !dgate)))
+        return -2;
+    if (!post_codes || !post_bytes || (post_g && !post_rstd) || (pre_g && (!gh || ldgh < W || !pre_codes || !pre_bytes || !pre_rstd))) return -2;
+    const size_t size = dtype == T8_F32 ? 4 : 2;
+    NjArgs a = {};
+    a.x = gy, a.f = gh, a.gate = gate, a.scale_v = scale_v, a.post_g = post_g, a.post_b = post_b, a.pre_g = pre_g, a.pre_b = pre_b, a.y = dx, a.h = df;
+    a.post_c = (unsigned char*)post_codes, a.post_e = (unsigned char*)post_bytes, a.pre_c = (unsigned char*)pre_codes, a.pre_e = (unsigned char*)pre_bytes;
+    a.post_r = (float*)post_rstd, a.pre_r = (float*)pre_rstd, a.dgate = dgate, a.part = workspace;
+    a.M = M, a.ldx = ldgy, a.ldf = ldgh, a.ldg = ldg, a.ldy = W, a.ldh = W, a.rows_per_gate = gate ? M / G : M, a.W = W, a.layer = layer;
+    a.has_post = post_g != nullptr, a.has_pre = pre_g != nullptr, a.has_gate = gate != nullptr, a.scale = scale;
+    const void* p[] = {gy, pre_g ? gh : nullptr, gate, dx, df, dgate};
+    const long ld[] = {ldgy, ldgh, ldg, W, W, W};
+    a.vec = nj_vec(W, size, p, ld, 6);
+    const long grid = nj_bwd_grid(M, W, gate ? G : 0, &a.per_group);
+    a.groups = gate ? G : 1, a.own_group = gate && !a.per_group;
+    a.need_sums = a.per_group || d_scale || d_post_g || d_post_b || d_pre_g || d_pre_b;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == T8_F32) nj_backward<float>(a, dim3((unsigned)grid), st);
+    else nj_backward<__bf16>(a, dim3((unsigned)grid), st);
+    const dim3 pg((W + 31) / 32, a.per_group ? (unsigned)G : 1);
+    if (a.per_group) {
+        if (dtype == T8_F32) k_norm_join_gate<float><<<pg, 256, 0, st>>>(a);
+        else k_norm_join_gate<__bf16><<<pg, 256, 0, st>>>(a);
+    }
+    if (d_scale || d_post_g || d_post_b || d_pre_g || d_pre_b)
+        k_norm_join_params<<<dim3(pg.x), 256, 0, st>>>(a, a.per_group ? (int)G : (int)grid, a.per_group ? a.per_group : 1, d_scale, d_post_g, d_post_b, d_pre_g, d_pre_b);
+    return (int)hipGetLastError();
+}

@@ -780,6 +780,302 @@ def mpnn_readout_bwd(h, dout, tw, w1, b1, k1, s1, w2, k2, use_swish, dt):
     return dh, du, gp
 
 
+# ------------------------------------------------------------------------------------ 8-bit tape
+TAPE8_KINDS = {"signed": 0, "relu": 1}
+_T8_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_T8_ACTS = {"none": ACT_NONE, "relu": ACT_RELU, "swish": ACT_SWISH}
+NORM_JOIN_MAX_WIDTH = 4096
+
+
+@dataclass
+class Tape8:
+    """Activations kept in 8 bits (csrc/tape8.cuh): ``codes`` uint8 [M, 32 ceil(width / 32)] and one byte per block of 32 columns,
+    ``bytes`` uint8 [M, ceil(width / 32)]; value = code 2^(byte - 127).  ``kind``: "signed", or "relu" (codes 0 .. 255, 0 exactly where the
+    value was <= 0).  33 bytes for 32 values; a value comes back to half a step (relu: values under half a step to a whole one) of its
+    block, the step being at most 2 / 127 (2 / 255) of the block's largest magnitude."""
+    codes: torch.Tensor
+    bytes: torch.Tensor
+    width: int
+    kind: str = "signed"
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+
+def tape8_empty(rows: int, width: int, kind: str = "signed", device="cuda") -> Tape8:
+    """an uninitialised tape (``tape8_pack(out=...)``)"""
+    if kind not in TAPE8_KINDS or width < 1 or rows < 0:
+        raise ValueError(f"magnet_amd: no 8-bit tape of kind {kind!r}, {rows} rows, width {width}")
+    nb = (width + 31) // 32
+    return Tape8(torch.empty(rows, 32 * nb, dtype=torch.uint8, device=device), torch.empty(rows, nb, dtype=torch.uint8, device=device), width, kind)
+
+
+def _tape8_ok(t: Tape8, name="tape", kind=None, width=None, rows=None) -> Tape8:
+    if not isinstance(t, Tape8):
+        raise TypeError(f"magnet_amd: {name} must be an ops.Tape8 (got {type(t).__name__})")
+    nb = (t.width + 31) // 32
+    if t.kind not in TAPE8_KINDS or t.width < 1:
+        raise ValueError(f"magnet_amd: {name}: kind {t.kind!r}, width {t.width}")
+    for a, w in ((t.codes, 32 * nb), (t.bytes, nb)):
+        _is_tensor(a, name)
+        if a.dtype != torch.uint8 or a.dim() != 2 or a.shape[1] != w or a.shape[0] != t.codes.shape[0] or not a.is_contiguous():
+            raise ValueError(f"magnet_amd: {name}: a tape of width {t.width} is contiguous uint8 codes [M, {32 * nb}] and bytes [M, {nb}] "
+                             f"(got {tuple(t.codes.shape)} and {tuple(t.bytes.shape)})")
+    if t.codes.data_ptr() & 15:
+        raise ValueError(f"magnet_amd: {name}: the codes must be 16-byte aligned")
+    if kind is not None and t.kind != kind:
+        raise ValueError(f"magnet_amd: {name} is a {t.kind!r} tape, a {kind!r} one is needed")
+    if (width is not None and t.width != width) or (rows is not None and t.rows != rows):
+        raise ValueError(f"magnet_amd: {name} has {t.rows} rows of width {t.width}, expected {rows} of {width}")
+    return t
+
+
+def _is_tensor(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"magnet_amd: {name} must be a tensor (got {type(t).__name__})")
+
+
+def _on_device(**tensors):
+    """every tensor that is there lives on the current HIP device (checked last: a call that is wrong anyway says so on any machine)"""
+    for name, t in tensors.items():
+        for u in ((t.codes, t.bytes) if isinstance(t, Tape8) else (t,)):
+            if u is None:
+                continue
+            if not u.is_cuda:
+                raise RuntimeError(f"magnet_amd: {name} must live on a HIP device (got {u.device}); there is no CPU path")
+            _same_device(u, name)
+
+
+def _matrix(t, name, dtypes, shape=None):
+    """a 2-D tensor of one of ``dtypes`` whose rows are runs of neighbouring values (copied where they are not)"""
+    _is_tensor(t, name)
+    if t.dtype not in dtypes:
+        raise TypeError(f"magnet_amd: {name} is {t.dtype}; supported: {', '.join(str(d) for d in dtypes)}")
+    if t.dim() != 2 or t.shape[1] < 1 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"magnet_amd: {name} has shape {tuple(t.shape)}" + (f", expected {tuple(shape)}" if shape is not None else ", expected [rows, width >= 1]"))
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t):
+    """elements from one row to the next (of one row at least its width: torch reports any stride there)"""
+    return C.c_long(max(t.stride(0), t.shape[1]))
+
+
+def _out_matrix(t, name, dtype, shape, device):
+    """an output the caller handed in, as it is, or a new one"""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _is_tensor(t, name)
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or (t.stride(-1) != 1 and t.shape[-1] > 1) or \
+            (t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"magnet_amd: {name} must be {dtype} of shape {tuple(shape)} with neighbouring columns (got {t.dtype} {tuple(t.shape)}, strides {t.stride()})")
+    return t
+
+
+def _overlap(a, b):
+    """whether the memory that two tensors span has bytes in common"""
+    def span(t):
+        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def tape8_pack(x, kind="signed", out=None) -> Tape8:
+    """x [M, W] (fp32, bf16 or fp16) onto an 8-bit tape (csrc/tape8_kernels.hip)"""
+    if kind not in TAPE8_KINDS:
+        raise ValueError(f"magnet_amd: tape kind {kind!r}; supported: {', '.join(TAPE8_KINDS)}")
+    x = _matrix(x, "x", tuple(_T8_DTYPES))
+    M, W = x.shape
+    t = _tape8_ok(out, "out", kind, W, M) if out is not None else None
+    _on_device(x=x, out=t)
+    if t is None:
+        t = tape8_empty(M, W, kind, x.device)
+    L.check(L.lib().magnet_tape8_pack(_p(x), _T8_DTYPES[x.dtype], _ld(x), C.c_long(M), W, TAPE8_KINDS[kind], _p(t.codes), _p(t.bytes), _stream()), "tape8_pack")
+    return t
+
+
+def tape8_unpack(t: Tape8, dtype=torch.float32, out=None):
+    """what a tape stands for, [M, W] (all of fp32, bf16 and fp16 hold a code exactly; fp16 not every step)"""
+    _tape8_ok(t)
+    if dtype not in _T8_DTYPES:
+        raise TypeError(f"magnet_amd: a tape is read as {', '.join(str(d) for d in _T8_DTYPES)} (got {dtype})")
+    _on_device(tape=t)
+    y = _out_matrix(out, "out", dtype, (t.rows, t.width), t.codes.device)
+    _on_device(out=y)
+    L.check(L.lib().magnet_tape8_unpack(_p(t.codes), _p(t.bytes), C.c_long(t.rows), t.width, TAPE8_KINDS[t.kind], _p(y), _T8_DTYPES[dtype], _ld(y), _stream()),
+            "tape8_unpack")
+    return y
+
+
+def _floats(entry, *args):
+    n = C.c_long(0)
+    L.check(getattr(L.lib(), entry)(*args, C.byref(n)), entry)
+    return n.value
+
+
+def tape8_linear_bwd(dz, tape: Tape8, w, act="none", *, need_dx=True, dx=None, dW=None, db=None, accumulate=False):
+    """A Linear (weight ``w`` [N, K]) walked back from the 8-bit tape of its input, in one pass over the rows: with v the tape's values and
+    x = act(v), dx [M, K] = act'(v) (dz w), dW [N, K] (+)= dz^T x, db [N] (+)= column sums of dz -> (dx or None, dW, db).  ``act``: "none"
+    (signed tape of x), "relu" (relu tape of x), "swish" (signed tape of Swish's argument).  fp32; ``accumulate`` adds to the dW and db
+    that are handed in."""
+    if act not in _T8_ACTS:
+        raise ValueError(f"magnet_amd: act {act!r}; supported: {', '.join(_T8_ACTS)}")
+    w = _matrix(w, "w", (torch.float32,))
+    N, K = w.shape
+    dz = _matrix(dz, "dz", (torch.float32,))
+    M = dz.shape[0]
+    if dz.shape[1] != N:
+        raise ValueError(f"magnet_amd: dz has {dz.shape[1]} columns, w {N} rows")
+    _tape8_ok(tape, "tape", "relu" if act == "relu" else "signed", K, M)
+    if accumulate and (dW is None or db is None):
+        raise ValueError("magnet_amd: accumulate needs the dW and db to add to")
+    for o, name, shape in ((dx, "dx", (M, K)), (dW, "dW", (N, K)), (db, "db", (N,))):
+        if o is not None and _overlap(_out_matrix(o, name, torch.float32, shape, None), dz):
+            raise ValueError(f"magnet_amd: {name} must not overlap dz")
+    _on_device(dz=dz, tape=tape, w=w, dx=dx, dW=dW, db=db)
+    dev = dz.device
+    if need_dx and dx is None:
+        dx = torch.empty(M, K, dtype=torch.float32, device=dev)
+    dW = torch.empty(N, K, dtype=torch.float32, device=dev) if dW is None else dW
+    db = torch.empty(N, dtype=torch.float32, device=dev) if db is None else db
+    ws = torch.empty(max(_floats("magnet_tape8_linear_bwd_workspace", C.c_long(M), N, K), 1), device=dev, dtype=torch.float32)
+    L.check(L.lib().magnet_tape8_linear_bwd_f32(_p(dz), _ld(dz), _p(tape.codes), _p(tape.bytes), _p(w), _ld(w), C.c_long(M), N, K, _T8_ACTS[act],
+                                                _p(dx), _ld(dx) if dx is not None else C.c_long(0), _p(dW), _ld(dW), _p(db), int(bool(accumulate)), _p(ws),
+                                                _stream()), "tape8_linear_bwd")
+    return dx, dW, db
+
+
+# ------------------------------------------------------------------------------------ norms around a residual block
+@dataclass
+class NormJoin:
+    """what ``norm_join`` returns: y, h (None without a pre norm) and, with ``tape``, what ``norm_join_bwd`` reads"""
+    y: torch.Tensor
+    h: torch.Tensor | None
+    post_tape: Tape8 | None = None
+    post_rstd: torch.Tensor | None = None
+    pre_tape: Tape8 | None = None
+    pre_rstd: torch.Tensor | None = None
+
+
+@dataclass
+class NormJoinGrads:
+    """gradients of ``norm_join``: x, f, gate, scale and the (gain, bias) pairs post and pre; None for what was not there"""
+    x: torch.Tensor
+    f: torch.Tensor
+    gate: torch.Tensor | None = None
+    scale: torch.Tensor | None = None
+    post: tuple | None = None
+    pre: tuple | None = None
+
+
+def _vector(t, name, W):
+    if t is None:
+        return None
+    _is_tensor(t, name)
+    if t.dtype != torch.float32 or tuple(t.shape) != (W,):
+        raise ValueError(f"magnet_amd: {name} must be fp32 of shape ({W},) (got {t.dtype} {tuple(t.shape)})")
+    return t.contiguous()
+
+
+def _norm_pair(p, name, W):
+    if p is None:
+        return None, None
+    if not isinstance(p, (tuple, list)) or len(p) != 2 or p[0] is None:
+        raise ValueError(f"magnet_amd: {name} is (gain, bias) with bias None where there is none")
+    return _vector(p[0], name + " gain", W), _vector(p[1], name + " bias", W)
+
+
+def _join_args(x, name, post, pre, gate, scale, norm):
+    """checks what both directions take -> (x, post pair, pre pair, gate, G, scale vector, scale number)"""
+    x = _matrix(x, name, (torch.float32, torch.bfloat16))
+    M, W = x.shape
+    if W > NORM_JOIN_MAX_WIDTH:
+        raise ValueError(f"magnet_amd: norm_join takes rows of at most {NORM_JOIN_MAX_WIDTH} values (got {W})")
+    if norm not in ("layer", "rms"):
+        raise ValueError(f"magnet_amd: norm {norm!r}; supported: layer, rms")
+    G = 0
+    if gate is not None:
+        _is_tensor(gate, "gate")
+        gate = _matrix(gate.unsqueeze(0) if gate.dim() == 1 else gate, "gate", (x.dtype,))
+        G = gate.shape[0]
+        if gate.shape[1] != W or G < 1 or M % G:
+            raise ValueError(f"magnet_amd: gate {tuple(gate.shape)} does not divide {M} rows of {W} values into equal runs")
+    vec = _vector(scale, "scale", W) if isinstance(scale, torch.Tensor) else None
+    return x, _norm_pair(post, "post", W), _norm_pair(pre, "pre", W), gate, G, vec, 0.0 if vec is not None else float(scale)
+
+
+def norm_join(x, f, *, post=None, pre=None, gate=None, scale=1.0, norm="layer", eps=1e-5, tape=False) -> NormJoin:
+    """The end of a residual block and the beginning of the next one in one pass (csrc/norm_join.hip):
+
+        y = x + scale * gate * post(f),   h = pre(y)
+
+    x, f [M, W <= 4096] fp32 or bf16.  ``post`` / ``pre``: (gain, bias or None) fp32 [W] of a norm of the kind ``norm`` ("layer" or "rms"),
+    or None: no such norm (no post: f itself; no pre: no h).  ``gate``: [G, W], M % G == 0 - row r takes gate[r // (M // G)]: one for every
+    element, one per graph of a batch, or one ([W]) for all.  ``scale``: a number or fp32 [W].  ``tape``: keep what ``norm_join_bwd``
+    needs - both normalised rows in 8 bits, 1 / sqrt(variance + eps) in fp32."""
+    x, (pg, pb), (qg, qb), gate, G, sv, sc = _join_args(x, "x", post, pre, gate, scale, norm)
+    M, W = x.shape
+    f = _matrix(f, "f", (x.dtype,), (M, W))
+    _on_device(x=x, f=f, post=pg, post_bias=pb, pre=qg, pre_bias=qb, gate=gate, scale=sv)
+    dev = x.device
+    r = NormJoin(torch.empty(M, W, dtype=x.dtype, device=dev), torch.empty(M, W, dtype=x.dtype, device=dev) if qg is not None else None)
+    if tape:
+        r.post_tape = tape8_empty(M, W, "signed", dev)
+        if pg is not None:
+            r.post_rstd = torch.empty(M, dtype=torch.float32, device=dev)
+        if qg is not None:
+            r.pre_tape, r.pre_rstd = tape8_empty(M, W, "signed", dev), torch.empty(M, dtype=torch.float32, device=dev)
+    pt, qt = r.post_tape, r.pre_tape
+    L.check(L.lib().magnet_norm_join(_p(x), _ld(x), _p(f), _ld(f), _T8_DTYPES[x.dtype], C.c_long(M), W, int(norm == "layer"), C.c_float(float(eps)),
+                                     _p(pg), _p(pb), _p(qg), _p(qb), _p(gate), _ld(gate) if gate is not None else C.c_long(0), C.c_long(G), _p(sv),
+                                     C.c_float(sc), _p(r.y), _p(r.h), _p(pt.codes if pt else None), _p(pt.bytes if pt else None), _p(r.post_rstd),
+                                     _p(qt.codes if qt else None), _p(qt.bytes if qt else None), _p(r.pre_rstd), _stream()), "norm_join")
+    return r
+
+
+def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_rstd=None, post=None, pre=None, gate=None, scale=1.0,
+                  norm="layer") -> NormJoinGrads:
+    """The backward pass of ``norm_join`` from the gradients of y and h (with a pre norm) and what its ``tape`` kept; post, pre, gate, scale and
+    norm as handed to it.  Gradients of x, f and gate have gy's type, those of parameters are fp32."""
+    gy, (pg, pb), (qg, qb), gate, G, sv, sc = _join_args(gy, "gy", post, pre, gate, scale, norm)
+    M, W = gy.shape
+    if (gh is None) != (qg is None):
+        raise ValueError("magnet_amd: gh is the gradient of h: it comes with a pre norm, and only with one")
+    gh = _matrix(gh, "gh", (gy.dtype,), (M, W)) if gh is not None else None
+    _tape8_ok(post_tape, "post_tape", "signed", W, M)
+    if qg is not None:
+        _tape8_ok(pre_tape, "pre_tape", "signed", W, M)
+    for v, name, need in ((post_rstd, "post_rstd", pg is not None), (pre_rstd, "pre_rstd", qg is not None)):
+        if need:
+            _is_tensor(v, name)
+            if v.dtype != torch.float32 or tuple(v.shape) != (M,) or not v.is_contiguous():
+                raise ValueError(f"magnet_amd: {name} must be contiguous fp32 of shape ({M},)")
+    _on_device(gy=gy, gh=gh, post=pg, post_bias=pb, pre=qg, pre_bias=qb, gate=gate, scale=sv, post_tape=post_tape,
+               post_rstd=post_rstd if pg is not None else None, pre_tape=pre_tape if qg is not None else None, pre_rstd=pre_rstd if qg is not None else None)
+    dev = gy.device
+    fill = torch.empty if M else torch.zeros                # (no rows: no launch)
+    new = lambda *s: fill(*s, dtype=gy.dtype, device=dev)  # noqa: E731
+    par = lambda p: fill(W, dtype=torch.float32, device=dev) if p is not None else None  # noqa: E731
+    g = NormJoinGrads(new(M, W), new(M, W), new(*gate.shape) if gate is not None else None, par(sv),
+                      (par(pg), par(pb)) if pg is not None else None, (par(qg), par(qb)) if qg is not None else None)
+    if M == 0:
+        return g
+    ws = torch.empty(_floats("magnet_norm_join_bwd_workspace", C.c_long(M), W, C.c_long(G)), device=dev, dtype=torch.float32)
+    post_g, pre_g = g.post or (None, None), g.pre or (None, None)
+    L.check(L.lib().magnet_norm_join_bwd(_p(gy), _ld(gy), _p(gh), _ld(gh) if gh is not None else C.c_long(0), _T8_DTYPES[gy.dtype], C.c_long(M), W,
+                                         int(norm == "layer"), _p(pg), _p(pb), _p(qg), _p(qb), _p(gate), _ld(gate) if gate is not None else C.c_long(0),
+                                         C.c_long(G), _p(sv), C.c_float(sc), _p(post_tape.codes), _p(post_tape.bytes),
+                                         _p(post_rstd if pg is not None else None), _p(pre_tape.codes if qg is not None else None),
+                                         _p(pre_tape.bytes if qg is not None else None), _p(pre_rstd if qg is not None else None), _p(g.x), _p(g.f),
+                                         _p(g.gate), _p(g.scale), _p(post_g[0]), _p(post_g[1]), _p(pre_g[0]), _p(pre_g[1]), _p(ws), _stream()),
+            "norm_join_bwd")
+    return g
+
+
 # ------------------------------------------------------------------------------------ graphs
 @dataclass
 class CSR:

@@ -1,0 +1,135 @@
+"""What the 8-bit tape's operators refuse, on any machine: nothing here launches a kernel (every wrong call is found before the device is
+looked at, and a right one on the CPU ends with "no CPU path")."""
+import pytest
+import torch
+
+from magnet_amd import _lib, ops
+
+
+def tape(M, W, kind="signed"):
+    return ops.tape8_empty(M, W, kind, "cpu")
+
+
+def test_right_calls_need_a_device():
+    x = torch.randn(4, 40)
+    for call in (lambda: ops.tape8_pack(x), lambda: ops.tape8_unpack(tape(4, 40)),
+                 lambda: ops.tape8_linear_bwd(torch.randn(4, 8), tape(4, 40), torch.randn(8, 40)),
+                 lambda: ops.norm_join(x, x, post=(torch.ones(40), None), norm="rms"),
+                 lambda: ops.norm_join_bwd(x, post_tape=tape(4, 40))):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def test_pack_refusals():
+    with pytest.raises(ValueError, match="kind"):
+        ops.tape8_pack(torch.randn(4, 4), "unsigned")
+    with pytest.raises(TypeError, match="float64"):
+        ops.tape8_pack(torch.randn(4, 4, dtype=torch.float64))
+    with pytest.raises(TypeError, match="tensor"):
+        ops.tape8_pack([[1.0]])
+    for shape in ((4,), (2, 3, 4), (4, 0)):
+        with pytest.raises(ValueError, match="shape"):
+            ops.tape8_pack(torch.randn(*shape))
+    with pytest.raises(ValueError, match="kind|tape"):
+        ops.tape8_pack(torch.randn(4, 4), "relu", out=tape(4, 4))
+    with pytest.raises(ValueError, match="expected 4 of 4"):
+        ops.tape8_pack(torch.randn(4, 4), out=tape(5, 4))
+    with pytest.raises(ValueError):
+        ops.tape8_empty(4, 0)
+
+
+def test_unpack_refusals():
+    with pytest.raises(TypeError, match="Tape8"):
+        ops.tape8_unpack(torch.zeros(4, 4))
+    with pytest.raises(TypeError, match="float64"):
+        ops.tape8_unpack(tape(4, 4), dtype=torch.float64)
+    good = tape(4, 40)
+    for bad in (ops.Tape8(good.codes[:, :32], good.bytes, 40), ops.Tape8(good.codes, good.bytes[:3], 40), ops.Tape8(good.codes.float(), good.bytes, 40),
+                ops.Tape8(good.codes, good.bytes, 70), ops.Tape8(good.codes, good.bytes, 40, "other"),
+                ops.Tape8(torch.empty(4 * 64 + 1, dtype=torch.uint8)[1:].view(4, 64), good.bytes, 40)):
+        with pytest.raises(ValueError):
+            ops.tape8_unpack(bad)
+
+
+def test_linear_bwd_refusals():
+    dz, w = torch.randn(6, 8), torch.randn(8, 40)
+    go = ops.tape8_linear_bwd
+    with pytest.raises(ValueError, match="act"):
+        go(dz, tape(6, 40), w, act="gelu")
+    with pytest.raises(ValueError, match="'relu'"):
+        go(dz, tape(6, 40), w, act="relu")
+    with pytest.raises(ValueError, match="'signed'"):
+        go(dz, tape(6, 40, "relu"), w)
+    with pytest.raises(ValueError, match="columns"):
+        go(dz[:, :7], tape(6, 40), w)
+    with pytest.raises(ValueError, match="expected 6 of 40"):
+        go(dz, tape(6, 41), w)
+    with pytest.raises(ValueError, match="expected 6 of 40"):
+        go(dz, tape(5, 40), w)
+    with pytest.raises(TypeError, match="bfloat16"):
+        go(dz.bfloat16(), tape(6, 40), w)
+    with pytest.raises(ValueError, match="accumulate"):
+        go(dz, tape(6, 40), w, accumulate=True)
+    for kw in (dict(dx=torch.empty(6, 41)), dict(dW=torch.empty(40, 8)), dict(db=torch.empty(9)), dict(dW=torch.empty(40, 8).t()),
+               dict(dx=torch.empty(6, 40, dtype=torch.float16))):
+        with pytest.raises(ValueError):
+            go(dz, tape(6, 40), w, **kw)
+    big = torch.randn(6, 80)
+    with pytest.raises(ValueError, match="overlap"):
+        go(big[:, 20:60], tape(6, 40), torch.randn(40, 40), dx=big[:, :40])
+
+
+def test_norm_join_refusals():
+    x = torch.randn(6, 40)
+    g, b = torch.ones(40), torch.zeros(40)
+    with pytest.raises(ValueError, match="at most"):
+        ops.norm_join(torch.randn(2, 4097), torch.randn(2, 4097))
+    with pytest.raises(ValueError, match="norm 'batch'"):
+        ops.norm_join(x, x, norm="batch")
+    with pytest.raises(TypeError, match="float16"):
+        ops.norm_join(x.half(), x.half())
+    with pytest.raises(TypeError, match="bfloat16"):
+        ops.norm_join(x, x.bfloat16())
+    with pytest.raises(ValueError, match="expected"):
+        ops.norm_join(x, x[:5])
+    for bad in (g, (None, b), (g,), (g[:39], b), (g.double(), b), (g, b[:39])):
+        with pytest.raises(ValueError):
+            ops.norm_join(x, x, post=bad)
+    for gate in (torch.ones(4, 40), torch.ones(6, 39), torch.ones(0, 40), torch.ones(12, 40)):
+        with pytest.raises(ValueError):
+            ops.norm_join(x, x, gate=gate)
+    with pytest.raises(TypeError):
+        ops.norm_join(x, x, gate=torch.ones(6, 40).bfloat16())
+    with pytest.raises(ValueError, match="scale"):
+        ops.norm_join(x, x, scale=torch.ones(()))
+    t, r = tape(6, 40), torch.ones(6)
+    with pytest.raises(ValueError, match="gh"):
+        ops.norm_join_bwd(x, x, post_tape=t)
+    with pytest.raises(ValueError, match="gh"):
+        ops.norm_join_bwd(x, post_tape=t, pre=(g, b))
+    with pytest.raises(TypeError, match="pre_tape"):
+        ops.norm_join_bwd(x, x, post_tape=t, pre=(g, b))
+    with pytest.raises(TypeError, match="post_rstd"):
+        ops.norm_join_bwd(x, post_tape=t, post=(g, b))
+    with pytest.raises(ValueError, match="post_rstd"):
+        ops.norm_join_bwd(x, post_tape=t, post=(g, b), post_rstd=r[:5])
+    with pytest.raises(ValueError, match="expected 6 of 40"):
+        ops.norm_join_bwd(x, post_tape=tape(6, 72))
+
+
+def test_c_entries_refuse():
+    """the C entries check what they can by themselves: -2, nothing launched (no device here)"""
+    import ctypes as C
+    L = _lib.lib()
+    z, one, n = C.c_void_p(0), C.c_void_p(16), C.c_long(0)
+    long = C.c_long
+    assert L.magnet_tape8_pack(one, 3, long(4), long(1), 4, 0, one, one, z) == -2          # no such type
+    assert L.magnet_tape8_pack(one, 0, long(3), long(1), 4, 0, one, one, z) == -2          # stride under the width
+    assert L.magnet_tape8_pack(one, 0, long(4), long(1), 4, 2, one, one, z) == -2          # no such kind
+    assert L.magnet_tape8_pack(one, 0, long(4), long(1), 4, 0, C.c_void_p(8), one, z) == -2
+    assert L.magnet_tape8_pack(one, 0, long(4), long(0), 4, 0, one, one, z) == 0           # no rows: nothing to do
+    assert L.magnet_tape8_unpack(one, one, long(-1), 4, 0, one, 0, long(4), z) == -2
+    assert L.magnet_tape8_linear_bwd_workspace(long(100), 0, 4, C.byref(n)) == -2
+    assert L.magnet_tape8_linear_bwd_workspace(long(100), 128, 128, C.byref(n)) == 0 and n.value == 4 * (128 * 128 + 128)
+    assert L.magnet_norm_join_bwd_workspace(long(100), 128, long(3), C.byref(n)) == -2      # 3 gates for 100 rows
+    assert L.magnet_norm_join_bwd_workspace(long(100), 4097, long(0), C.byref(n)) == -2
