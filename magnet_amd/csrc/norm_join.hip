@@ -13,11 +13,14 @@
 //     d pre_gain = sum gh y^; d pre_bias = sum gh                                            ([mean u]: LayerNorm only)
 // All four sums over rows are linear in  S1 = sum gate D f^,  S0 = sum gate D,  P1 = sum gh y^,  P0 = sum gh  - four sums per column.
 //
-// Both are bound by HBM: every array is read or written once.  A row belongs to a team of 16 to 256 lanes, four neighbouring columns per
-// lane and slot, and stays in registers from its load to its last use; statistics are lane exchanges (through LDS for a team of four
-// waves), fp32, the variance around the mean.  Gradients of parameters: a lane adds its columns over the rows that its team walks, teams
-// and workgroups are added in their order (the same bits every time).
+// Both are bound by HBM: every array is read or written once.  A row belongs to a team of 16 to 512 lanes, four neighbouring columns per
+// lane and slot, at most two slots: it stays in registers from its load to its last use, and the next row of the team is loaded before this
+// one is worked on (the statistics are two dependent sums over the row: without rows in flight behind them the loads' latency is what
+// the kernel takes).  Sums over a team are lane exchanges inside the vector unit, through LDS for a team of several waves; fp32, the
+// variance around the mean.  Gradients of parameters: a lane adds its columns over the rows that its team walks, teams and workgroups are
+// added in their order (the same bits every time).
 #include "common.cuh"
+#include "split_single.cuh"
 #include "tape8.cuh"
 
 struct NjArgs {
@@ -31,53 +34,104 @@ struct NjArgs {
     long M, ldx, ldf, ldg, ldy, ldh;
     long rows_per_gate;                  // M / G (M without a gate)
     long groups;                         // backward: G, 1 without a gate
-    int W, vec, layer, has_post, has_pre, has_gate, tape, per_group, own_group, need_sums;
+    int W, vec, layer, has_post, has_pre, has_gate, tape, per_group, need_sums;
     float scale, eps;
 };
 
-// sum over a team of TL lanes (a team of 256: the whole workgroup, through LDS)
-template <int TL>
-__device__ __forceinline__ float nj_sum(float v, float* red) {
-    constexpr int L = TL < 64 ? TL : 64;
-#pragma unroll
-    for (int o = L / 2; o; o >>= 1) v += __shfl_xor(v, o);
-    if (TL > 64) {
-        __syncthreads();
-        if (!(threadIdx.x & 63)) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = (red[0] + red[1]) + (red[2] + red[3]);
+// sums over a team of TL lanes: neighbours, quads, halves of 16 by lane permutes of the vector unit, then rows of 16 and halves of the wave
+template <int CTRL>
+__device__ __forceinline__ float nj_dpp(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+template <int L>
+__device__ __forceinline__ float nj_lanes(float v) {
+    v = nj_dpp<0xB1>(v);                                                      // quad_perm 1 0 3 2
+    v = nj_dpp<0x4E>(v);                                                      // quad_perm 2 3 0 1
+    v = nj_dpp<0x141>(v);                                                     // row_half_mirror: the other four of eight
+    v = nj_dpp<0x140>(v);                                                     // row_mirror: the other eight of sixteen
+    if (L > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        const unsigned r0 = r[0], r1 = r[1];                                  // (a bit cast of r[1] itself reads r[0])
+        v = __uint_as_float(r0) + __uint_as_float(r1);
+    }
+    if (L > 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        const unsigned r0 = r[0], r1 = r[1];                                  // (a bit cast of r[1] itself reads r[0])
+        v = __uint_as_float(r0) + __uint_as_float(r1);
     }
     return v;
+}
+struct NjRed {                           // the meeting place of a team of several waves: two sums, two places used in turn (one barrier per sum:
+    float v[2][2][8];                    // between two uses of a place lies the barrier of the other)
+};
+template <int TL, bool BOTH>
+__device__ __forceinline__ void nj_sum(float& a, float& b, NjRed& red, int& turn) {
+    a = nj_lanes<(TL < 64 ? TL : 64)>(a);
+    if (BOTH) b = nj_lanes<(TL < 64 ? TL : 64)>(b);
+    if (TL > 64) {
+        constexpr int NW = TL / 64;
+        if (!(threadIdx.x & 63)) {
+            red.v[turn][0][threadIdx.x >> 6] = a;
+            if (BOTH) red.v[turn][1][threadIdx.x >> 6] = b;
+        }
+        wg_barrier();
+        a = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) a += red.v[turn][0][w];
+        if (BOTH) {
+            b = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) b += red.v[turn][1][w];
+        }
+        turn ^= 1;
+    }
 }
 __device__ __forceinline__ float nj_hsum(const t8_f4& v) { return (v[0] + v[1]) + (v[2] + v[3]); }
 __device__ __forceinline__ float nj_dot(const t8_f4& a, const t8_f4& b) { return (a[0] * b[0] + a[1] * b[1]) + (a[2] * b[2] + a[3] * b[3]); }
 
 // v -> (v - mean) r or v r in place; returns r.  Columns past the width hold zero before and after.
 template <int TL, int VPT>
-__device__ __forceinline__ float nj_norm(t8_f4 (&v)[VPT], int lane, int W, int layer, float eps, float* red) {
-    const float inv = 1.0f / (float)W;
-    if (layer) {
+__device__ __forceinline__ float nj_norm(t8_f4 (&v)[VPT], int lane, const NjArgs& a, NjRed& red, int& turn) {
+    const float inv = 1.0f / (float)a.W;
+    float none = 0.f;
+    if (a.layer) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) s += nj_hsum(v[i]);
-        const float mean = nj_sum<TL>(s, red) * inv;
+        nj_sum<TL, false>(s, none, red, turn);
+        s *= inv;
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[i][c] = 4 * (i * TL + lane) + c < W ? v[i][c] - mean : 0.f;
+            for (int c = 0; c < 4; ++c) v[i][c] = 4 * (i * TL + lane) + c < a.W ? v[i][c] - s : 0.f;
     }
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) q += nj_dot(v[i], v[i]);
-    const float r = 1.0f / sqrtf(nj_sum<TL>(q, red) * inv + eps);
+    nj_sum<TL, false>(q, none, red, turn);
+    const float r = 1.0f / sqrtf(q * inv + a.eps);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) v[i] *= r;
     return r;
 }
+// u (times r) without its part along v^ (and, LayerNorm, without its mean): the gradient at a norm's input
+template <int TL, int VPT>
+__device__ __forceinline__ void nj_norm_bwd(t8_f4 (&u)[VPT], const t8_f4 (&vh)[VPT], float r, int lane, const NjArgs& a, NjRed& red, int& turn) {
+    const float inv = 1.0f / (float)a.W;
+    float s = 0.f, p = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) s += nj_hsum(u[i]), p += nj_dot(u[i], vh[i]);
+    nj_sum<TL, true>(p, s, red, turn);
+    p *= inv;
+    s = a.layer ? s * inv : 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) u[i][c] = 4 * (i * TL + lane) + c < a.W ? ((u[i][c] - s) - vh[i][c] * p) * r : 0.f;
+}
 // the normalised row onto the tape
 template <int TL, int VPT>
-__device__ __forceinline__ void nj_tape(const t8_f4 (&v)[VPT], int lane, int W, long row, unsigned char* codes, unsigned char* bytes) {
-    const int blocks = (W + 31) / 32;
+__device__ __forceinline__ void nj_tape(const t8_f4 (&v)[VPT], int lane, int blocks, long row, unsigned char* codes, unsigned char* bytes) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int c = 4 * (i * TL + lane);
@@ -88,16 +142,7 @@ __device__ __forceinline__ void nj_tape(const t8_f4 (&v)[VPT], int lane, int W, 
         }
     }
 }
-template <int TL, int VPT>
-__device__ __forceinline__ void nj_untape(t8_f4 (&v)[VPT], int lane, int W, long row, const unsigned char* codes, const unsigned char* bytes) {
-    const int blocks = (W + 31) / 32;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int c = 4 * (i * TL + lane);
-        v[i] = c < W ? t8_decode4<T8_SIGNED>(*reinterpret_cast<const unsigned*>(codes + row * (32 * blocks) + c), bytes[row * blocks + c / 32]) : t8_f4{0.f, 0.f, 0.f, 0.f};
-    }
-}
-// a row of parameters (fp32, any alignment of the row's columns past the width reads zero)
+// a row of parameters: fp32, zero past the width; `none` where there is none
 __device__ __forceinline__ t8_f4 nj_par(const float* p, int c, int W, float none) {
     t8_f4 v = {none, none, none, none};
     if (!p) return v;
@@ -105,158 +150,199 @@ __device__ __forceinline__ t8_f4 nj_par(const float* p, int c, int W, float none
     for (int i = 0; i < 4; ++i) v[i] = c + i < W ? p[c + i] : 0.f;
     return v;
 }
-
 __device__ __forceinline__ t8_f4 nj_scale(const NjArgs& a, int c) {
     return a.scale_v ? nj_par(a.scale_v, c, a.W, 0.f) : t8_f4{a.scale, a.scale, a.scale, a.scale};
 }
+// four neighbouring values as they are in memory (a row in flight)
+template <typename T>
+using nj_raw = T __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ nj_raw<T> nj_load(const T* __restrict__ p, bool vec, int n) {
+    if (vec) return n > 0 ? *reinterpret_cast<const nj_raw<T>*>(p) : nj_raw<T>(0);
+    nj_raw<T> v = nj_raw<T>(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < n) v[i] = p[i];
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ t8_f4 nj_f32(const nj_raw<T>& v) { return t8_f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}; }
 
 template <typename T, int TL, int VPT>
-__global__ void __launch_bounds__(256) k_norm_join(const NjArgs a) {
-    __shared__ float red[4];
-    constexpr int TEAMS = 256 / TL;
-    const int lane = threadIdx.x % TL;
-    const int W = a.W;
+__global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join(const NjArgs a) {
+    __shared__ NjRed red;
+    constexpr int TEAMS = (TL > 256 ? TL : 256) / TL;
+    const int lane = threadIdx.x % TL, W = a.W, blocks = (W + 31) / 32;
     const T *x = (const T*)a.x, *f = (const T*)a.f, *gate = (const T*)a.gate;
     T *y = (T*)a.y, *h = (T*)a.h;
-    // (every lane of a wave walks as often as its neighbours: the lane exchanges need them all; rows past the end are clamped and not stored)
+    int turn = 0;
+    t8_f4 sc[VPT], pg[VPT], pb[VPT], qg[VPT], qb[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int c = 4 * (i * TL + lane);
+        sc[i] = nj_scale(a, c);
+        pg[i] = nj_par(a.post_g, c, W, 1.f), pb[i] = nj_par(a.post_b, c, W, 0.f);
+        qg[i] = nj_par(a.pre_g, c, W, 1.f), qb[i] = nj_par(a.pre_b, c, W, 0.f);
+    }
+    // the team's rows, and the gate row of each: advanced by the stride, split once into gate rows and the rest
     const long stride = (long)gridDim.x * TEAMS;
-    for (long base = (long)blockIdx.x * TEAMS; base < a.M; base += stride) {
-        const long row = base + threadIdx.x / TL;
-        const bool on = row < a.M;
-        const long r = on ? row : a.M - 1;
-        t8_f4 v[VPT], s[VPT];
+    long row = (long)blockIdx.x * TEAMS + threadIdx.x / TL;
+    long g = row / a.rows_per_gate, in_g = row - g * a.rows_per_gate;
+    const long dg = stride / a.rows_per_gate, din = stride - dg * a.rows_per_gate;
+    nj_raw<T> nx[VPT], nf[VPT], ng[VPT];
+    auto load = [&](long r, long gr) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            v[i] = t8_load4(f + r * a.ldf + c, a.vec && c < W, W - c);
-            s[i] = t8_load4(x + r * a.ldx + c, a.vec && c < W, W - c);
+            nf[i] = nj_load(f + r * a.ldf + c, a.vec, W - c);
+            nx[i] = nj_load(x + r * a.ldx + c, a.vec, W - c);
+            if (a.has_gate) ng[i] = nj_load(gate + gr * a.ldg + c, a.vec, W - c);
         }
+    };
+    if (row < a.M) load(row, g);
+    for (; row < a.M; row += stride) {
+        t8_f4 v[VPT], s[VPT], m[VPT];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            v[i] = nj_f32<T>(nf[i]), s[i] = nj_f32<T>(nx[i]);
+            m[i] = a.has_gate ? sc[i] * nj_f32<T>(ng[i]) : sc[i];
+        }
+        g += dg, in_g += din;
+        if (in_g >= a.rows_per_gate) in_g -= a.rows_per_gate, ++g;
+        if (row + stride < a.M) load(row + stride, g);
         if (a.has_post) {
-            const float rs = nj_norm<TL, VPT>(v, lane, W, a.layer, a.eps, red);
-            if (a.tape && on && lane == 0) a.post_r[row] = rs;
+            const float rs = nj_norm<TL, VPT>(v, lane, a, red, turn);
+            if (a.tape && lane == 0) a.post_r[row] = rs;
         }
-        if (a.tape && on) nj_tape<TL, VPT>(v, lane, W, row, a.post_c, a.post_e);
-        const long gr = a.has_gate ? r / a.rows_per_gate : 0;
+        if (a.tape) nj_tape<TL, VPT>(v, lane, blocks, row, a.post_c, a.post_e);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            t8_f4 t = v[i];
-            if (a.has_post) {
-                t = t * nj_par(a.post_g, c, W, 1.f);
-                if (a.post_b) t += nj_par(a.post_b, c, W, 0.f);
-            }
-            if (a.has_gate) t *= t8_load4(gate + gr * a.ldg + c, a.vec && c < W, W - c);
-            s[i] += nj_scale(a, c) * t;
-            if (on) t8_store4(y + r * a.ldy + c, a.vec && c < W, W - c, s[i]);
+            s[i] += m[i] * (v[i] * pg[i] + pb[i]);                            // (gain one, bias zero where there is none)
+            t8_store4(y + row * a.ldy + c, a.vec, W - c, s[i]);
         }
         if (!a.has_pre) continue;
         // (the second norm reads y before it is rounded to T)
-        const float rs = nj_norm<TL, VPT>(s, lane, W, a.layer, a.eps, red);
-        if (a.tape && on && lane == 0) a.pre_r[row] = rs;
-        if (a.tape && on) nj_tape<TL, VPT>(s, lane, W, row, a.pre_c, a.pre_e);
+        const float rs = nj_norm<TL, VPT>(s, lane, a, red, turn);
+        if (a.tape) {
+            if (lane == 0) a.pre_r[row] = rs;
+            nj_tape<TL, VPT>(s, lane, blocks, row, a.pre_c, a.pre_e);
+        }
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            t8_f4 t = s[i] * nj_par(a.pre_g, c, W, 1.f);
-            if (a.pre_b) t += nj_par(a.pre_b, c, W, 0.f);
-            if (on) t8_store4(h + r * a.ldh + c, a.vec && c < W, W - c, t);
+            t8_store4(h + row * a.ldh + c, a.vec, W - c, s[i] * qg[i] + qb[i]);
         }
     }
-}
-
-// u (times r) without its part along v^ (and, LayerNorm, without its mean): the gradient at a norm's input
-template <int TL, int VPT>
-__device__ __forceinline__ void nj_norm_bwd(t8_f4 (&u)[VPT], const t8_f4 (&vh)[VPT], float r, int lane, int W, int layer, float* red) {
-    const float inv = 1.0f / (float)W;
-    float s = 0.f, p = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) s += nj_hsum(u[i]), p += nj_dot(u[i], vh[i]);
-    p = nj_sum<TL>(p, red) * inv;
-    s = layer ? nj_sum<TL>(s, red) * inv : 0.f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) u[i][c] = 4 * (i * TL + lane) + c < W ? ((u[i][c] - s) - vh[i][c] * p) * r : 0.f;
 }
 
 // Which rows a team walks, and where the sums of a gate row meet:
 //   no gate:          any rows, one set of sums for the launch
 //   G gate rows, few: per_group workgroups for each, their sums stay apart (S1, S0 without the gate) and meet in k_norm_join_gate
-//   many (own_group): a team takes whole gate rows one after the other - up to one for every row - and writes their gradients itself
-template <typename T, int TL, int VPT>
-__global__ void __launch_bounds__(256) k_norm_join_bwd(const NjArgs a) {
-    __shared__ float red[4];
-    __shared__ __attribute__((aligned(16))) float part[TL < 256 ? 256 * 4 : 4];
-    constexpr int TEAMS = 256 / TL;
-    const int lane = threadIdx.x % TL, team = threadIdx.x / TL;
-    const int W = a.W;
+//   many (OWN):       a team takes whole gate rows one after the other - up to one for every row - and writes their gradients itself
+template <typename T, int TL, int VPT, bool OWN>
+__global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjArgs a) {
+    __shared__ NjRed red;
+    constexpr int NT = TL > 256 ? TL : 256, TEAMS = NT / TL;
+    __shared__ __attribute__((aligned(16))) float part[TEAMS > 1 ? NT * 4 : 4];
+    const int lane = threadIdx.x % TL, team = threadIdx.x / TL, W = a.W, blocks = (W + 31) / 32;
     const T *gy = (const T*)a.x, *gh = (const T*)a.f, *gate = (const T*)a.gate;
     T *dx = (T*)a.y, *df = (T*)a.h, *dgate = (T*)a.dgate;
-    const long me = (long)blockIdx.x * TEAMS + team;
-    const long g_step = a.own_group ? (long)gridDim.x * TEAMS : a.groups;
-    t8_f4 S1[VPT], S0[VPT], P1[VPT], P0[VPT];
+    int turn = 0;
+    t8_f4 sc[VPT], pg[VPT], pb[VPT], qg[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) S1[i] = S0[i] = P1[i] = P0[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
-    for (long g = a.own_group ? me : a.per_group ? blockIdx.x / a.per_group : 0; g < a.groups; g += g_step) {
-        const long last = (g + 1) * a.rows_per_gate;
-        long row = g * a.rows_per_gate, step = 1;
-        if (!a.own_group) {
-            row += a.per_group ? (long)(blockIdx.x % a.per_group) * TEAMS + team : me;
-            step = (long)(a.per_group ? a.per_group : gridDim.x) * TEAMS;
-        }
-        t8_f4 T1[VPT], T0[VPT];
+    for (int i = 0; i < VPT; ++i) {
+        const int c = 4 * (i * TL + lane);
+        sc[i] = nj_scale(a, c);
+        pg[i] = nj_par(a.post_g, c, W, 1.f), qg[i] = nj_par(a.pre_g, c, W, 1.f);
+        if (OWN) pb[i] = nj_par(a.post_b, c, W, 0.f);
+    }
+    // this team's rows: `row`, then row + step up to the gate row's last; OWN: then the gate row g + g_step
+    const long me = (long)blockIdx.x * TEAMS + team, g_step = (long)gridDim.x * TEAMS;
+    long g = OWN ? me : a.per_group ? blockIdx.x / a.per_group : 0;
+    const long step = OWN ? 1 : (long)(a.per_group ? a.per_group : gridDim.x) * TEAMS;
+    long row = g * a.rows_per_gate + (OWN ? 0 : a.per_group ? (long)(blockIdx.x % a.per_group) * TEAMS + team : me);
+    long last = min(g + 1, a.groups) * a.rows_per_gate;
+    bool more = g < a.groups && row < last;
+    nj_raw<T> ny[VPT], nh[VPT], ng[VPT];
+    unsigned npc[VPT], nqc[VPT], npe[VPT], nqe[VPT];
+    float npr = 1.f, nqr = 1.f;
+    auto load = [&](long r, long gr) {
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) T1[i] = T0[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
-        for (; row < last; row += step) {
-            t8_f4 D[VPT], v[VPT];
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int c = 4 * (i * TL + lane);
-                D[i] = t8_load4(gy + row * a.ldx + c, a.vec && c < W, W - c);
-            }
-            if (a.has_pre) {
-                t8_f4 u[VPT];
-                nj_untape<TL, VPT>(v, lane, W, row, a.pre_c, a.pre_e);
-#pragma unroll
-                for (int i = 0; i < VPT; ++i) {
-                    const int c = 4 * (i * TL + lane);
-                    u[i] = t8_load4(gh + row * a.ldf + c, a.vec && c < W, W - c);
-                    P0[i] += u[i], P1[i] += u[i] * v[i];
-                    u[i] *= nj_par(a.pre_g, c, W, 1.f);
+        for (int i = 0; i < VPT; ++i) {
+            const int c = 4 * (i * TL + lane);
+            ny[i] = nj_load(gy + r * a.ldx + c, a.vec, W - c);
+            if (a.has_pre) nh[i] = nj_load(gh + r * a.ldf + c, a.vec, W - c);
+            if (a.has_gate) ng[i] = nj_load(gate + gr * a.ldg + c, a.vec, W - c);
+            npc[i] = npe[i] = nqc[i] = nqe[i] = 0u;
+            if (c < W) {
+                npc[i] = *reinterpret_cast<const unsigned*>(a.post_c + r * (32 * blocks) + c);
+                npe[i] = a.post_e[r * blocks + c / 32];
+                if (a.has_pre) {
+                    nqc[i] = *reinterpret_cast<const unsigned*>(a.pre_c + r * (32 * blocks) + c);
+                    nqe[i] = a.pre_e[r * blocks + c / 32];
                 }
-                nj_norm_bwd<TL, VPT>(u, v, a.pre_r[row], lane, W, a.layer, red);
-#pragma unroll
-                for (int i = 0; i < VPT; ++i) D[i] += u[i];
             }
-            nj_untape<TL, VPT>(v, lane, W, row, a.post_c, a.post_e);
+        }
+        if (a.has_post) npr = a.post_r[r];
+        if (a.has_pre) nqr = a.pre_r[r];
+    };
+    t8_f4 S1[VPT], S0[VPT], P1[VPT], P0[VPT], T1[VPT], T0[VPT];               // T: of the gate row so far, without the gate
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) S1[i] = S0[i] = P1[i] = P0[i] = T1[i] = T0[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
+    if (more) load(row, g);
+    while (more) {
+        t8_f4 D[VPT], v[VPT], gt[VPT], u[VPT], q[VPT];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            D[i] = nj_f32<T>(ny[i]);
+            v[i] = t8_decode4<T8_SIGNED>(npc[i], npe[i]);
+            gt[i] = a.has_gate ? nj_f32<T>(ng[i]) : t8_f4{1.f, 1.f, 1.f, 1.f};
+            if (a.has_pre) u[i] = nj_f32<T>(nh[i]), q[i] = t8_decode4<T8_SIGNED>(nqc[i], nqe[i]);
+        }
+        const float pr = npr, qr = nqr;
+        // the row after this one, on its way while this one is worked on
+        const long r = row, gr = g;
+        row += step;
+        bool ends = false;
+        if (row >= last) {
+            ends = true;
+            if (OWN) {
+                g += g_step;
+                row = g * a.rows_per_gate, last = row + a.rows_per_gate;
+                more = g < a.groups;
+            } else {
+                more = false;
+            }
+        }
+        if (more) load(row, g);
+        if (a.has_pre) {
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
-                const int c = 4 * (i * TL + lane);
-                t8_store4(dx + row * a.ldy + c, a.vec && c < W, W - c, D[i]);
-                T0[i] += D[i], T1[i] += D[i] * v[i];
-                if (a.has_gate) D[i] *= t8_load4(gate + g * a.ldg + c, a.vec && c < W, W - c);
-                D[i] *= nj_scale(a, c);
-                if (a.has_post) D[i] *= nj_par(a.post_g, c, W, 1.f);
+                P0[i] += u[i], P1[i] += u[i] * q[i];
+                u[i] *= qg[i];
             }
-            if (a.has_post) nj_norm_bwd<TL, VPT>(D, v, a.post_r[row], lane, W, a.layer, red);
+            nj_norm_bwd<TL, VPT>(u, q, qr, lane, a, red, turn);
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int c = 4 * (i * TL + lane);
-                t8_store4(df + row * a.ldh + c, a.vec && c < W, W - c, D[i]);
-            }
+            for (int i = 0; i < VPT; ++i) D[i] += u[i];
         }
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            t8_f4 gt = {1.f, 1.f, 1.f, 1.f};
-            if (a.own_group) {
-                const int c = 4 * (i * TL + lane);
-                gt = t8_load4(gate + g * a.ldg + c, a.vec && c < W, W - c);
-                t8_f4 t = T1[i];
-                if (a.has_post) t *= nj_par(a.post_g, c, W, 1.f);
-                if (a.post_b) t += T0[i] * nj_par(a.post_b, c, W, 0.f);
-                t8_store4(dgate + g * W + c, a.vec && c < W, W - c, t * nj_scale(a, c));
+            const int c = 4 * (i * TL + lane);
+            t8_store4(dx + r * a.ldy + c, a.vec, W - c, D[i]);
+            T0[i] += D[i], T1[i] += D[i] * v[i];
+            D[i] *= gt[i] * sc[i] * pg[i];
+        }
+        if (a.has_post) nj_norm_bwd<TL, VPT>(D, v, pr, lane, a, red, turn);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = 4 * (i * TL + lane);
+            t8_store4(df + r * a.ldh + c, a.vec, W - c, D[i]);
+            if (OWN && ends) {
+                t8_store4(dgate + gr * W + c, a.vec, W - c, (T1[i] * pg[i] + T0[i] * pb[i]) * sc[i]);
+                S1[i] += gt[i] * T1[i], S0[i] += gt[i] * T0[i];
+                T1[i] = T0[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
             }
-            S1[i] += gt * T1[i], S0[i] += gt * T0[i];
         }
     }
     if (!a.need_sums) return;
@@ -266,7 +352,7 @@ __global__ void __launch_bounds__(256) k_norm_join_bwd(const NjArgs a) {
     for (int q = 0; q < 4; ++q)
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            t8_f4 s = q == 0 ? S1[i] : q == 1 ? S0[i] : q == 2 ? P1[i] : P0[i];
+            t8_f4 s = q == 0 ? (OWN ? S1[i] : T1[i]) : q == 1 ? (OWN ? S0[i] : T0[i]) : q == 2 ? P1[i] : P0[i];
             const int c = 4 * (i * TL + lane);
             if (TEAMS > 1) {
                 __syncthreads();
@@ -284,7 +370,7 @@ __global__ void __launch_bounds__(256) k_norm_join_bwd(const NjArgs a) {
         }
 }
 
-// sums of a column over n of the workgroups' sets (`first`, first + apart, ..), in order: a workgroup takes 32 columns, eight slices of the sets each; the total in
+// sums of a column over n of the workgroups' sets (`first`, first + apart, ..), in order: a workgroup takes 32 columns, 32 slices of the sets each; the total in
 // v of slice 0
 __device__ __forceinline__ void nj_fold(const float* part, long first, int n, long apart, int W, int c, float (&v)[4], float (*s)[4][32]) {
     const int col = threadIdx.x & 31, slice = threadIdx.x >> 5;
@@ -292,7 +378,7 @@ __device__ __forceinline__ void nj_fold(const float* part, long first, int n, lo
     for (int q = 0; q < 4; ++q) v[q] = 0.f;
     if (c < W)
 #pragma unroll 4
-        for (int w = slice; w < n; w += 8) {
+        for (int w = slice; w < n; w += 32) {
             const float* p = part + (first + w * apart) * 4 * W + c;
 #pragma unroll
             for (int q = 0; q < 4; ++q) v[q] += p[(long)q * W];
@@ -304,13 +390,13 @@ __device__ __forceinline__ void nj_fold(const float* part, long first, int n, lo
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         v[q] = s[0][q][col];
-        for (int k = 1; k < 8; ++k) v[q] += s[k][q][col];
+        for (int k = 1; k < 32; ++k) v[q] += s[k][q][col];
     }
 }
 // one gate row (blockIdx.y): its gradient, and its workgroups' sums with the gate multiplied in, left in the first one's place
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_join_gate(const NjArgs a) {
-    __shared__ float s[8][4][32];
+__global__ void __launch_bounds__(1024) k_norm_join_gate(const NjArgs a) {
+    __shared__ float s[32][4][32];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), W = a.W;
     const long g = blockIdx.y;
     float v[4];
@@ -323,9 +409,9 @@ __global__ void __launch_bounds__(256) k_norm_join_gate(const NjArgs a) {
     p[0] = gt * v[0], p[W] = gt * v[1], p[2 * W] = v[2], p[3 * W] = v[3];
 }
 // the parameters' gradients from n sets of sums, `apart` sets from one to the next
-__global__ void __launch_bounds__(256) k_norm_join_params(const NjArgs a, int n, int apart, float* d_scale, float* d_post_g, float* d_post_b, float* d_pre_g,
+__global__ void __launch_bounds__(1024) k_norm_join_params(const NjArgs a, int n, int apart, float* d_scale, float* d_post_g, float* d_post_b, float* d_pre_g,
                                                           float* d_pre_b) {
-    __shared__ float s[8][4][32];
+    __shared__ float s[32][4][32];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31);
     float v[4];
     nj_fold(a.part, 0, n, apart, a.W, c, v, s);
@@ -340,16 +426,18 @@ __global__ void __launch_bounds__(256) k_norm_join_params(const NjArgs a, int n,
 
 // ---------------------------------------------------------------------------------------------------------------------------- launches
 #define NJ_MAX_W 4096
-static int nj_team(int W) { return W <= 64 ? 16 : W <= 128 ? 32 : W <= 1024 ? 64 : 256; }
+// lanes of a row's team: two slots of four columns each, sixteen lanes at least
+static int nj_team(int W) { return W <= 128 ? 16 : W <= 256 ? 32 : W <= 512 ? 64 : W <= 2048 ? 256 : 512; }
+static int nj_teams(int W) { return W <= 2048 ? 256 / nj_team(W) : 1; }
 static long nj_grid(long M, int W) {
-    const int teams = 256 / nj_team(W);
+    const int teams = nj_teams(W);
     const long n = (M + teams - 1) / teams;
-    return n < 2048 ? n : 2048;
+    return n < 1024 ? n : 1024;
 }
 // backward: workgroups, and how many of them share a gate row (0: they are not bound to gate rows).  Up to 2048 gate rows get workgroups of
 // their own - a set of sums each, added by a second launch; beyond that a team walks whole gate rows and no sums are kept per row
 static long nj_bwd_grid(long M, int W, long G, int* per_group) {
-    const int teams = 256 / nj_team(W);
+    const int teams = nj_teams(W);
     *per_group = 0;
     if (G <= 0 || G > 2048 || G == M) {
         const long n = ((G > 2048 ? G : M) + teams - 1) / teams;
@@ -371,23 +459,23 @@ static void nj_forward(const NjArgs& a, hipStream_t st) {
     const dim3 grid((unsigned)nj_grid(a.M, a.W));
     const int W = a.W;
     if (W <= 64) k_norm_join<T, 16, 1><<<grid, 256, 0, st>>>(a);
-    else if (W <= 128) k_norm_join<T, 32, 1><<<grid, 256, 0, st>>>(a);
-    else if (W <= 256) k_norm_join<T, 64, 1><<<grid, 256, 0, st>>>(a);
+    else if (W <= 128) k_norm_join<T, 16, 2><<<grid, 256, 0, st>>>(a);
+    else if (W <= 256) k_norm_join<T, 32, 2><<<grid, 256, 0, st>>>(a);
     else if (W <= 512) k_norm_join<T, 64, 2><<<grid, 256, 0, st>>>(a);
-    else if (W <= 1024) k_norm_join<T, 64, 4><<<grid, 256, 0, st>>>(a);
+    else if (W <= 1024) k_norm_join<T, 256, 1><<<grid, 256, 0, st>>>(a);
     else if (W <= 2048) k_norm_join<T, 256, 2><<<grid, 256, 0, st>>>(a);
-    else k_norm_join<T, 256, 4><<<grid, 256, 0, st>>>(a);
+    else k_norm_join<T, 512, 2><<<grid, 512, 0, st>>>(a);
 }
-template <typename T>
+template <typename T, bool OWN>
 static void nj_backward(const NjArgs& a, dim3 grid, hipStream_t st) {
     const int W = a.W;
-    if (W <= 64) k_norm_join_bwd<T, 16, 1><<<grid, 256, 0, st>>>(a);
-    else if (W <= 128) k_norm_join_bwd<T, 32, 1><<<grid, 256, 0, st>>>(a);
-    else if (W <= 256) k_norm_join_bwd<T, 64, 1><<<grid, 256, 0, st>>>(a);
-    else if (W <= 512) k_norm_join_bwd<T, 64, 2><<<grid, 256, 0, st>>>(a);
-    else if (W <= 1024) k_norm_join_bwd<T, 64, 4><<<grid, 256, 0, st>>>(a);
-    else if (W <= 2048) k_norm_join_bwd<T, 256, 2><<<grid, 256, 0, st>>>(a);
-    else k_norm_join_bwd<T, 256, 4><<<grid, 256, 0, st>>>(a);
+    if (W <= 64) k_norm_join_bwd<T, 16, 1, OWN><<<grid, 256, 0, st>>>(a);
+    else if (W <= 128) k_norm_join_bwd<T, 16, 2, OWN><<<grid, 256, 0, st>>>(a);
+    else if (W <= 256) k_norm_join_bwd<T, 32, 2, OWN><<<grid, 256, 0, st>>>(a);
+    else if (W <= 512) k_norm_join_bwd<T, 64, 2, OWN><<<grid, 256, 0, st>>>(a);
+    else if (W <= 1024) k_norm_join_bwd<T, 256, 1, OWN><<<grid, 256, 0, st>>>(a);
+    else if (W <= 2048) k_norm_join_bwd<T, 256, 2, OWN><<<grid, 256, 0, st>>>(a);
+    else k_norm_join_bwd<T, 512, 2, OWN><<<grid, 512, 0, st>>>(a);
 }
 static int nj_vec(int W, size_t size, const void* const* p, const long* ld, int n) {
     int ok = !(W & 3);
@@ -439,17 +527,18 @@ extern "C" int magnet_norm_join_bwd(const void* gy, long ldgy, const void* gh, l
     const long ld[] = {ldgy, ldgh, ldg, W, W, W};
     a.vec = nj_vec(W, size, p, ld, 6);
     const long grid = nj_bwd_grid(M, W, gate ? G : 0, &a.per_group);
-    a.groups = gate ? G : 1, a.own_group = gate && !a.per_group;
+    a.groups = gate ? G : 1;
     a.need_sums = a.per_group || d_scale || d_post_g || d_post_b || d_pre_g || d_pre_b;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == T8_F32) nj_backward<float>(a, dim3((unsigned)grid), st);
-    else nj_backward<__bf16>(a, dim3((unsigned)grid), st);
+    const bool own = gate && !a.per_group;
+    if (dtype == T8_F32) own ? nj_backward<float, true>(a, dim3((unsigned)grid), st) : nj_backward<float, false>(a, dim3((unsigned)grid), st);
+    else own ? nj_backward<__bf16, true>(a, dim3((unsigned)grid), st) : nj_backward<__bf16, false>(a, dim3((unsigned)grid), st);
     const dim3 pg((W + 31) / 32, a.per_group ? (unsigned)G : 1);
     if (a.per_group) {
-        if (dtype == T8_F32) k_norm_join_gate<float><<<pg, 256, 0, st>>>(a);
-        else k_norm_join_gate<__bf16><<<pg, 256, 0, st>>>(a);
+        if (dtype == T8_F32) k_norm_join_gate<float><<<pg, 1024, 0, st>>>(a);
+        else k_norm_join_gate<__bf16><<<pg, 1024, 0, st>>>(a);
     }
     if (d_scale || d_post_g || d_post_b || d_pre_g || d_pre_b)
-        k_norm_join_params<<<dim3(pg.x), 256, 0, st>>>(a, a.per_group ? (int)G : (int)grid, a.per_group ? a.per_group : 1, d_scale, d_post_g, d_post_b, d_pre_g, d_pre_b);
+        k_norm_join_params<<<dim3(pg.x), 1024, 0, st>>>(a, a.per_group ? (int)G : (int)grid, a.per_group ? a.per_group : 1, d_scale, d_post_g, d_post_b, d_pre_g, d_pre_b);
     return (int)hipGetLastError();
 }

@@ -107,9 +107,9 @@ __device__ __forceinline__ t8_f4 t8_decode4(unsigned w, unsigned byte) {
     const float s = t8_step(byte);
     return t8_f4{t8_q<KIND>(w, 0) * s, t8_q<KIND>(w, 1) * s, t8_q<KIND>(w, 2) * s, t8_q<KIND>(w, 3) * s};
 }
-// the top of a block of 32 columns: eight neighbouring lanes hold four columns each
+// the top of a block of 32 columns: eight neighbouring lanes hold four columns each (quad_perm 1 0 3 2, 2 3 0 1, row_half_mirror)
 __device__ __forceinline__ unsigned t8_max8(unsigned t) {
-    t = max(t, (unsigned)__shfl_xor((int)t, 1));
-    t = max(t, (unsigned)__shfl_xor((int)t, 2));
-    return max(t, (unsigned)__shfl_xor((int)t, 4));
+    t = max(t, (unsigned)__builtin_amdgcn_update_dpp(0, (int)t, 0xB1, 0xF, 0xF, true));
+    t = max(t, (unsigned)__builtin_amdgcn_update_dpp(0, (int)t, 0x4E, 0xF, 0xF, true));
+    return max(t, (unsigned)__builtin_amdgcn_update_dpp(0, (int)t, 0x141, 0xF, 0xF, true));
 }

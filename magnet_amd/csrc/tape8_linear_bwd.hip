@@ -12,16 +12,17 @@
 // The error of both is a few 2^-22 of the operands' magnitude, sums are held in fp32, and the workgroups' partial sums of dW and db are added
 // in their order by a second kernel: the same bits every time.
 //
-// Scales.  fp16 spans 2^40; gradients (1e-7) and tapes (any byte) do not fit by themselves.  The workgroup keeps the largest exponent it
-// has met, of dz and of the tape's bytes, and stages everything times the power of two that puts it at the top of the range; a step that
-// brings a larger one scales the sums down first.  Rows 2^-30 below the largest so far start to lose bits, of a share that small of the sums.
-// A wave scales its own part of W likewise.
+// Scales.  fp16 spans 2^40; gradients (1e-7) and tapes (any byte) do not fit by themselves.  The workgroup keeps a bound on the exponents it has
+// met, of dz and of the tape's bytes, and stages everything times the power of two that puts the bound near the top of the range.  A lane
+// that meets more raises a flag with its write; behind the barrier that the step has anyway all waves see it, add their sums so far to the
+// workgroup's partial sums in memory and begin again under a new bound (with a few binades to spare): rare after the first step, and
+// nobody waits for a maximum otherwise.  (Scaling the sums in registers instead costs a second set of them: measured as spills.)  Rows 2^-24 below the largest so far start to lose bits, of a share that small of the sums.  A wave scales its part of W likewise.
 #include "common.cuh"
 #include "split_single.cuh"
 #include "tape8.cuh"
 
 typedef _Float16 t8_h8 __attribute__((ext_vector_type(8)));
-typedef __fp16 t8_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 t8_hp __attribute__((ext_vector_type(2)));
 typedef short t8_s4 __attribute__((__vector_size__(4 * sizeof(short))));
 
 struct T8LinArgs {
@@ -37,68 +38,136 @@ struct T8LinArgs {
 };
 
 // exponent byte (1 .. 254) of a magnitude's bits; 0 for zero, subnormals and what is not finite
-__device__ __forceinline__ unsigned t8_expo(unsigned m) {
-    const unsigned e = m >> 23;
+__device__ __forceinline__ unsigned t8_expo(float v) {
+    const unsigned e = (__float_as_uint(v) >> 23) & 0xFFu;
     return e == 255u ? 0u : e;
 }
 __device__ __forceinline__ float t8_pow2(int biased) { return __uint_as_float((unsigned)min(max(biased, 0), 254) << 23); }
-// two values as one word of each fp16 plane: h towards zero, l = what is left, to nearest
-__device__ __forceinline__ void t8_split(float a, float b, unsigned& h, unsigned& l) {
-    const t8_h2 hh = __builtin_amdgcn_cvt_pkrtz(a, b);
-    const _Float16 la = (_Float16)(a - (float)hh[0]), lb = (_Float16)(b - (float)hh[1]);
-    h = __builtin_bit_cast(unsigned, hh);
-    l = (unsigned)__builtin_bit_cast(unsigned short, la) | (unsigned)__builtin_bit_cast(unsigned short, lb) << 16;
-}
 // four halfwords of a column out of a 16 x 4 tile: lane i of 16 points at row i / 4, columns 4 (i % 4) .., and gets column i
 __device__ __forceinline__ t8_u2 t8_tr(const unsigned short* p) {
     return __builtin_bit_cast(t8_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) t8_s4*)(p)));
 }
 __device__ __forceinline__ t8_h8 t8_join(t8_u2 a, t8_u2 b) { return __builtin_bit_cast(t8_h8, t8_u4{a[0], a[1], b[0], b[1]}); }
-// Swish and its derivative: s = sigmoid(v); v s and s (1 + v (1 - s))
-__device__ __forceinline__ float t8_sigmoid(float v) { return 1.0f / (1.0f + __expf(-v)); }
+// e^-v (finite: past 87 both s and what is left of it are under 2^-125) and s = 1 / (1 + e^-v)
+__device__ __forceinline__ float t8_sigmoid(float v, float& e) {
+    e = __expf(fminf(-v, 87.0f));
+    return __builtin_amdgcn_rcpf(1.0f + e);
+}
+__device__ __forceinline__ float t8_swish(float v) {
+    float e;
+    return v * t8_sigmoid(v, e);
+}
+// Swish's derivative s (1 + v (1 - s)) with 1 - s = e^-v s: no cancellation where s is near 1
 __device__ __forceinline__ float t8_dswish(float v) {
-    const float s = t8_sigmoid(v);
-    return s + v * s * t8_sigmoid(-v);   // (1 - s as a sigmoid: no cancellation where s is near 1)
+    float e;
+    const float s = t8_sigmoid(v, e);
+    return s + v * s * (e * s);
 }
 
-template <int NP, int KP, int ACT>
-__global__ void __launch_bounds__(256, 2) k_tape8_linear_bwd(const T8LinArgs a) {
+#define T8_WAVES(NP, KP) ((NP) == 128 && (KP) == 128 ? 8 : 4)
+#define T8_ZROOM 3                       // binades of dz and of the tape's bytes that may still come before the scale has to change
+#define T8_XROOM 2
+template <int NP, int KP, int XPL>
+struct T8Step {                          // a step of 32 rows in LDS; row strides of 16 halfwords more than a power of two spread the rows over the banks
+    unsigned short z[2][32][NP + 16];
+    unsigned short x[XPL][32][KP + 16];
+    unsigned c[32][KP / 4 + 4];          // the codes (the mask; Swish's argument)
+    unsigned char b[32][KP / 32];
+};
+
+// a value at a wave-uniform base plus the lane's offset in bytes (global_* with a scalar base: the caller hides the base behind an asm statement,
+// or the compiler adds the two and keeps 64 bits per lane and access in registers)
+template <typename V>
+__device__ __forceinline__ V t8_at(const void* base, unsigned off) {
+    return *reinterpret_cast<__attribute__((address_space(1))) const V*>((__attribute__((address_space(1))) const char*)(base) + off);
+}
+template <typename V>
+__device__ __forceinline__ void t8_put(void* base, unsigned off, const V& v) {
+    *reinterpret_cast<__attribute__((address_space(1))) V*>((__attribute__((address_space(1))) char*)(base) + off) = v;
+}
+#define T8_UNIFORM(p) asm volatile("" : "+s"(p))
+
+// FULL: N = NP, K a multiple of KP, dz and dx in 16-byte accesses, one block of N - no lane ever looks at a column that is not there, and
+// addresses are a uniform base and one offset (the registers that bounds and addresses take are what decides between spilling and not)
+// A workgroup of NP and KP at most 64 has four waves, else eight: a wave owns one block of 16 features of either side (of 64 features on
+// one side, every other wave the rows' other half).
+template <int NP, int KP, int ACT, bool FULL>
+__global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ? 4 : 2) k_tape8_linear_bwd(const T8LinArgs a) {
     constexpr int KIND = ACT == ACT_RELU ? T8_RELU : T8_SIGNED;
     constexpr int XPL = ACT == ACT_SWISH ? 2 : 1;                             // planes of x
-    constexpr int NST = NP + 16, KST = KP + 16, CST = KP / 4 + 4;             // row strides: halfwords, halfwords, words (bank spread)
-    constexpr int LPR = NP / 4, NLD = 32 * LPR / 256;                         // lanes per row of dz, rows of dz per lane
-    constexpr int CPR = KP / 16;                                              // lanes per row of codes (16 codes each)
-    constexpr int NBK = KP / 64, NBN = NP / 64, NT = NP / 32, KB = KP / 16;   // a wave's blocks of 16 features of x / of dz
-    __shared__ __attribute__((aligned(16))) unsigned short zi[2][32][NST];
-    __shared__ __attribute__((aligned(16))) unsigned short xi[XPL][32][KST];
-    __shared__ __attribute__((aligned(16))) unsigned ci[32][CST];
-    __shared__ unsigned char bi[32][KP / 32];
-    __shared__ unsigned red[4];
+    constexpr int NBUF = XPL == 2 && NP == 128 && KP == 128 ? 1 : 2;          // (two such steps for two workgroups a CU are more than 160 KB)
+    constexpr int NW = T8_WAVES(NP, KP), LANES = 64 * NW;
+    constexpr int LPR = NP / 4, RPL = LANES / LPR, NLD = 32 / RPL;            // lanes per row of dz, rows per pass, passes
+    constexpr int CPT = 32 * KP / LANES, CPR = KP / CPT, CW = CPT / 4;        // codes per lane (8 or 16), lanes per row, words
+    constexpr int NBK = KP / 16 / NW, NBN = NP / 16 / NW, NT = NP / 32, KB = KP / 16;   // a wave's blocks of 16 features of x / of dz
+    typedef unsigned t8_cw __attribute__((ext_vector_type(CW)));
+    __shared__ __attribute__((aligned(16))) T8Step<NP, KP, XPL> sb[NBUF];
+    __shared__ unsigned red[NW], flag[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
     const int k0 = blockIdx.y * KP;
+    // ---- what this lane loads of a step
+    const int zr = tid / LPR, zc = 4 * (tid % LPR);
+    const int cr = tid / CPR, cc = CPT * (tid % CPR);
+    const bool c_on = k0 + cc < a.ldc;
+    const int lb = a.ldc / 32;
+    t8_f4 dv[NLD];
+    t8_cw cv = t8_cw(0u);
+    unsigned bv = 0;
+    int shift = 0;                                                            // FULL, the last step: it takes the last 32 rows, this many of them done
+    auto load = [&](long step) {
+        if (FULL) {
+            const long row = min(step * 32, a.M - 32);
+            const unsigned oz = ((unsigned)zr * (unsigned)a.ldz + zc) * 4u, oc = (unsigned)cr * (unsigned)a.ldc + cc, ob = (unsigned)cr * (unsigned)lb + cc / 32;
+            const unsigned char *bc = a.codes + row * a.ldc + k0, *bb = a.bytes + row * lb + k0 / 32;
+            T8_UNIFORM(bc);
+            T8_UNIFORM(bb);
+#pragma unroll
+            for (int i = 0; i < NLD; ++i) {
+                const float* p = a.dz + (row + i * RPL) * a.ldz;
+                T8_UNIFORM(p);
+                dv[i] = t8_at<t8_f4>(p, oz);
+            }
+            cv = t8_at<t8_cw>(bc, oc), bv = t8_at<unsigned char>(bb, ob);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < NLD; ++i) {
+            const long r = step * 32 + zr + i * RPL;
+            dv[i] = r < a.M ? t8_load4(a.dz + r * a.ldz + zc, a.zvec && zc < a.N, a.N - zc) : t8_f4{0.f, 0.f, 0.f, 0.f};
+        }
+        const long r = step * 32 + cr;
+        const bool on = c_on && r < a.M;
+        cv = on ? *reinterpret_cast<const t8_cw*>(a.codes + r * a.ldc + k0 + cc) : t8_cw(0u);
+        bv = on ? a.bytes[r * lb + (k0 + cc) / 32] : 0u;
+    };
+    const long nsteps = (a.M + 31) / 32;
+    long step = blockIdx.x;
+    load(step);
     // ---- the wave's features of W^T: A operands (lane = feature of x, register j of k group q4 = feature 32 t + 8 q4 + j of dz)
     t8_h8 wh[NBK][NT], wl[NBK][NT];
-    float wscale;
+    int we;                                                                   // W is staged times 2^(140 - we): max |W| -> [2^13, 2^14)
     {
-        float wv[NBK][NT][8];
+        auto w_at = [&](int b, int t, int j) -> float {
+            const int n = 32 * t + 8 * q4 + j, k = k0 + 16 * (NBK * wave + b) + n16;
+            if (FULL) {
+                const float* p = a.w + (32 * t + j) * a.ldw + k0 + 16 * (NBK * wave + b);
+                T8_UNIFORM(p);
+                return t8_at<float>(p, ((unsigned)(8 * q4) * (unsigned)a.ldw + n16) * 4u);
+            }
+            return n < a.N && k < a.K ? a.w[n * a.ldw + k] : 0.f;
+        };
         unsigned top = 0;
 #pragma unroll
         for (int b = 0; b < NBK; ++b)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int n = 32 * t + 8 * q4 + j, k = k0 + 16 * (NBK * wave + b) + n16;
-                    const float v = n < a.N && k < a.K ? a.w[n * a.ldw + k] : 0.f;
-                    wv[b][t][j] = v;
-                    top = max(top, t8_expo(__float_as_uint(v) & 0x7FFFFFFFu));
-                }
+                for (int j = 0; j < 8; ++j) top = max(top, t8_expo(w_at(b, t, j)));
 #pragma unroll
         for (int o = 32; o; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
-        const int e = max((int)top, 14);
-        const float s = t8_pow2(267 - e);                                     // max |W| -> [2^13, 2^14)
-        wscale = t8_pow2(e - 13);
+        we = max(__builtin_amdgcn_readfirstlane((int)top), 14);
+        const float s = t8_pow2(267 - we);
 #pragma unroll
         for (int b = 0; b < NBK; ++b)
 #pragma unroll
@@ -107,112 +176,106 @@ __global__ void __launch_bounds__(256, 2) k_tape8_linear_bwd(const T8LinArgs a) 
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     unsigned hw, lw;
-                    t8_split(wv[b][t][2 * j] * s, wv[b][t][2 * j + 1] * s, hw, lw);
+                    split_f16_prod(w_at(b, t, 2 * j), s, w_at(b, t, 2 * j + 1), s, hw, lw);
                     h[j] = hw, l[j] = lw;
                 }
                 wh[b][t] = __builtin_bit_cast(t8_h8, h), wl[b][t] = __builtin_bit_cast(t8_h8, l);
             }
     }
-    // ---- what this lane loads of a step
-    const int zr = tid / LPR, zc = 4 * (tid % LPR);
-    const int cr = tid / CPR, cc = 16 * (tid % CPR);
-    const bool c_on = cr < 32 && k0 + cc < a.ldc;
-    const int lb = a.ldc / 32;
-    t8_f4 dv[NLD];
-    t8_u4 cv = {0u, 0u, 0u, 0u};
-    unsigned bv = 0;
-    auto load = [&](long step) {
+    t8_f4 bsum = {0.f, 0.f, 0.f, 0.f};
+    int ze = 14, xe = 8;                                                      // bounds: dz is staged times 2^(140 - ze), codes times 2^(byte - xe + 5)
+    // ---- this lane's part of the step in its two images; true if something lies above the bounds
+    auto stage = [&](T8Step<NP, KP, XPL>& B) -> bool {
+        float m = 0.f;
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
-            const long r = step * 32 + zr + i * (256 / LPR);
-            dv[i] = r < a.M ? t8_load4(a.dz + r * a.ldz + zc, a.zvec && zc < a.N, a.N - zc) : t8_f4{0.f, 0.f, 0.f, 0.f};
+            const float G = FULL && zr + i * RPL < shift ? 0.f : t8_pow2(267 - ze);
+            t8_u2 h, l;
+            unsigned hw, lw;
+            m = fmaxf(fmaxf(fmaxf(m, fabsf(dv[i][0])), fabsf(dv[i][1])), fmaxf(fabsf(dv[i][2]), fabsf(dv[i][3])));
+            split_f16_prod(dv[i][0], G, dv[i][1], G, hw, lw);
+            h[0] = hw, l[0] = lw;
+            split_f16_prod(dv[i][2], G, dv[i][3], G, hw, lw);
+            h[1] = hw, l[1] = lw;
+            *reinterpret_cast<t8_u2*>(&B.z[0][zr + i * RPL][zc]) = h;
+            *reinterpret_cast<t8_u2*>(&B.z[1][zr + i * RPL][zc]) = l;
         }
-        const long r = step * 32 + cr;
-        const bool on = c_on && r < a.M;
-        cv = on ? *reinterpret_cast<const t8_u4*>(a.codes + r * a.ldc + k0 + cc) : t8_u4{0u, 0u, 0u, 0u};
-        bv = on ? a.bytes[r * lb + (k0 + cc) / 32] : 0u;
+        const bool bad = bv == 255u;
+        unsigned p[XPL][2 * CW];
+        if (ACT == ACT_SWISH) {
+            const float up = t8_pow2(259 - xe);
+#pragma unroll
+            for (int j = 0; j < CW; ++j) {
+                const t8_f4 v = t8_decode4<KIND>(cv[j], bv);
+                split_f16_prod(t8_swish(v[0]), up, t8_swish(v[1]), up, p[0][2 * j], p[XPL - 1][2 * j]);
+                split_f16_prod(t8_swish(v[2]), up, t8_swish(v[3]), up, p[0][2 * j + 1], p[XPL - 1][2 * j + 1]);
+            }
+        } else {
+            // byte c beside 0x64 is the fp16 number 1024 + c (signed: c + 128 after the sign bit is turned): times the power of two, less what it
+            // is too much - one fused multiply-add for two codes, exact
+            const _Float16 s = bad ? __builtin_bit_cast(_Float16, (unsigned short)0x7E00) : (_Float16)t8_pow2((int)bv - xe + 132);
+            const _Float16 o = (KIND == T8_RELU ? (_Float16)-1024.0f : (_Float16)-1152.0f) * s;
+            const t8_hp s2 = {s, s}, o2 = {o, o};
+#pragma unroll
+            for (int j = 0; j < CW; ++j) {
+                const unsigned w = KIND == T8_RELU ? cv[j] : cv[j] ^ 0x80808080u;
+                p[0][2 * j] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(t8_hp, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)), s2, o2));
+                p[0][2 * j + 1] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(t8_hp, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)), s2, o2));
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < XPL; ++q)
+#pragma unroll
+            for (int j = 0; j < CPT / 8; ++j)
+                *reinterpret_cast<t8_u4*>(&B.x[q][cr][cc + 8 * j]) = t8_u4{p[q][4 * j], p[q][4 * j + 1], p[q][4 * j + 2], p[q][4 * j + 3]};
+        if (ACT != ACT_NONE) *reinterpret_cast<t8_cw*>(&B.c[cr][cc / 4]) = cv;
+        if (ACT == ACT_SWISH && !(cc & 31)) B.b[cr][cc / 32] = (unsigned char)bv;
+        return m >= t8_pow2(ze + 1) || (!bad && (int)bv > xe);
     };
-    f32x4 accw[NBN][KB];
-#pragma unroll
-    for (int b = 0; b < NBN; ++b)
-#pragma unroll
-        for (int x = 0; x < KB; ++x) accw[b][x] = f32x4{0.f, 0.f, 0.f, 0.f};
-    t8_f4 bsum = {0.f, 0.f, 0.f, 0.f};
-    int ze = 14, xe = 8;                                                      // largest exponents so far: of dz, and the largest byte
-    const long nsteps = (a.M + 31) / 32;
-    long step = blockIdx.x;
-    if (step < nsteps) load(step);
-    for (; step < nsteps; step += gridDim.x) {
-        // ---- the step's exponents
+    float* const wout = a.wpart + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * NP * KP;
+    bool first = true;
+    int it = 0;
+    while (step < nsteps) {              // one stretch of steps under the same bounds
         {
             unsigned m = 0;
 #pragma unroll
             for (int i = 0; i < NLD; ++i)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) m = max(m, t8_expo(__float_as_uint(dv[i][c]) & 0x7FFFFFFFu));
+                for (int c = 0; c < 4; ++c) m = max(m, t8_expo(dv[i][c]));
             unsigned mx = bv == 255u ? 0u : bv;
 #pragma unroll
             for (int o = 32; o; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o)), mx = max(mx, (unsigned)__shfl_xor((int)mx, o));
             if (lane == 0) red[wave] = m | mx << 8;
+            wg_barrier();
+            m = mx = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) m = max(m, red[w] & 0xFFu), mx = max(mx, red[w] >> 8);
+            ze = __builtin_amdgcn_readfirstlane((int)m > ze ? min((int)m + T8_ZROOM, 254) : ze);
+            xe = __builtin_amdgcn_readfirstlane((int)mx > xe ? (int)mx + T8_XROOM : xe);
+            if (tid < 2) flag[tid] = 0u;                                      // (everybody has read the flag that ended the last stretch)
         }
-        wg_barrier();                                                         // the exponents are there; the images have been read
-        {
-            unsigned m = 0, mx = 0;
+        f32x4 accw[NBN][KB];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) m = max(m, red[w] & 0xFFu), mx = max(mx, red[w] >> 8);
-            const int nz = max(ze, (int)m), nx = max(xe, (int)mx);
-            if (nz > ze || nx > xe) {                                         // (the same in every lane of the workgroup)
-                const float f = t8_pow2(127 + ze - nz) * t8_pow2(127 + xe - nx);
+        for (int b = 0; b < NBN; ++b)
 #pragma unroll
-                for (int b = 0; b < NBN; ++b)
-#pragma unroll
-                    for (int x = 0; x < KB; ++x) accw[b][x] *= f;
-                ze = nz, xe = nx;
-            }
-        }
-        const float G = t8_pow2(267 - ze);                                    // largest |dz| -> [2^13, 2^14)
-        // ---- the images
-#pragma unroll
-        for (int i = 0; i < NLD; ++i) {
-            t8_u2 h, l;
-            unsigned hw, lw;
-            bsum += dv[i];
-            t8_split(dv[i][0] * G, dv[i][1] * G, hw, lw);
-            h[0] = hw, l[0] = lw;
-            t8_split(dv[i][2] * G, dv[i][3] * G, hw, lw);
-            h[1] = hw, l[1] = lw;
-            *reinterpret_cast<t8_u2*>(&zi[0][zr + i * (256 / LPR)][zc]) = h;
-            *reinterpret_cast<t8_u2*>(&zi[1][zr + i * (256 / LPR)][zc]) = l;
-        }
-        if (cr < 32) {
-            // code * 2^(byte - xe + 7): at most 255 * 2^7; Swish of the value times the same power of two
-            const float xs = bv == 255u ? t8_step(255u) : ACT == ACT_SWISH ? t8_step(bv) : t8_pow2(bv == 0u ? 0 : (int)bv - xe + 134);
-            const float up = t8_pow2(261 - xe);
-            unsigned p[XPL][8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const unsigned w = cv[j >> 1];
-                float v0 = t8_q<KIND>(w, 2 * (j & 1)) * xs, v1 = t8_q<KIND>(w, 2 * (j & 1) + 1) * xs;
-                if (ACT == ACT_SWISH) {
-                    v0 = v0 * t8_sigmoid(v0) * up, v1 = v1 * t8_sigmoid(v1) * up;
-                    t8_split(v0, v1, p[0][j], p[XPL - 1][j]);
-                } else {
-                    p[0][j] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(v0, v1));
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < XPL; ++q) {
-                *reinterpret_cast<t8_u4*>(&xi[q][cr][cc]) = t8_u4{p[q][0], p[q][1], p[q][2], p[q][3]};
-                *reinterpret_cast<t8_u4*>(&xi[q][cr][cc + 8]) = t8_u4{p[q][4], p[q][5], p[q][6], p[q][7]};
-            }
-            if (ACT != ACT_NONE) *reinterpret_cast<t8_u4*>(&ci[cr][cc / 4]) = cv;
-            if (ACT == ACT_SWISH && !(cc & 16)) bi[cr][cc / 32] = (unsigned char)bv;
-        }
-        const long row0 = step * 32;
-        asm volatile("" ::: "memory");
-        if (step + gridDim.x < nsteps) load(step + gridDim.x);
-        asm volatile("" ::: "memory");
+            for (int x = 0; x < KB; ++x) accw[b][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // (a stretch's first step is what its bounds were made of: nothing to ask - and what is not finite would ask for more for ever)
+        for (bool fresh = true; step < nsteps; step += gridDim.x, ++it, fresh = false) {
+        T8Step<NP, KP, XPL>& B = sb[it & (NBUF - 1)];
+        if (NBUF == 1 && !fresh) wg_barrier();                                // the step before has been read
+        if (FULL) shift = (int)(step * 32 - min(step * 32, a.M - 32));
+        const bool over = stage(B);
+        if (!fresh && __any(over) && lane == 0) flag[it & 1] = 1u;
         wg_barrier();
+        if (!fresh && __builtin_amdgcn_readfirstlane((int)flag[it & 1])) break;     // (the same for every wave)
+#pragma unroll
+        for (int i = 0; i < NLD; ++i)
+            if (!FULL || zr + i * RPL >= shift) bsum += dv[i];
+        const long row0 = FULL ? min(step * 32, a.M - 32) : step * 32;
+        const int done = shift;
+        asm volatile("" ::: "memory");
+        load(min(step + (long)gridDim.x, nsteps - 1));                        // (past the last step: rows that nobody uses)
+        asm volatile("" ::: "memory");
         // ---- dx^T: acc[b][rb] = features 16 (NBK wave + b) .. of rows 16 rb ..
         f32x4 acc[NBK][2];
 #pragma unroll
@@ -221,8 +284,8 @@ __global__ void __launch_bounds__(256, 2) k_tape8_linear_bwd(const T8LinArgs a) 
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb) {
-                const t8_h8 zh = *reinterpret_cast<const t8_h8*>(&zi[0][16 * rb + n16][32 * t + 8 * q4]);
-                const t8_h8 zl = *reinterpret_cast<const t8_h8*>(&zi[1][16 * rb + n16][32 * t + 8 * q4]);
+                const t8_h8 zh = *reinterpret_cast<const t8_h8*>(&B.z[0][16 * rb + n16][32 * t + 8 * q4]);
+                const t8_h8 zl = *reinterpret_cast<const t8_h8*>(&B.z[1][16 * rb + n16][32 * t + 8 * q4]);
 #pragma unroll
                 for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl[b][t], zh, acc[b][rb], 0, 0, 0);
 #pragma unroll
@@ -230,6 +293,7 @@ __global__ void __launch_bounds__(256, 2) k_tape8_linear_bwd(const T8LinArgs a) 
 #pragma unroll
                 for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zh, acc[b][rb], 0, 0, 0);
             }
+        __builtin_amdgcn_sched_barrier(0);                                    // (without these the reads of all three parts move up and the registers run out)
         // ---- dW += dz^T x over the step's rows (k group q4: rows 4 q4 .. + 3 and 16 + 4 q4 .. + 3 of both operands)
         {
             const int r0 = 4 * q4 + (n16 >> 2), c0 = 4 * (n16 & 3);
@@ -237,14 +301,14 @@ __global__ void __launch_bounds__(256, 2) k_tape8_linear_bwd(const T8LinArgs a) 
 #pragma unroll
             for (int b = 0; b < NBN; ++b) {
                 const int f = 16 * (NBN * wave + b) + c0;
-                ah[b] = t8_join(t8_tr(&zi[0][r0][f]), t8_tr(&zi[0][16 + r0][f]));
-                al[b] = t8_join(t8_tr(&zi[1][r0][f]), t8_tr(&zi[1][16 + r0][f]));
+                ah[b] = t8_join(t8_tr(&B.z[0][r0][f]), t8_tr(&B.z[0][16 + r0][f]));
+                al[b] = t8_join(t8_tr(&B.z[1][r0][f]), t8_tr(&B.z[1][16 + r0][f]));
             }
 #pragma unroll
             for (int x = 0; x < KB; ++x) {
-                const t8_h8 xh = t8_join(t8_tr(&xi[0][r0][16 * x + c0]), t8_tr(&xi[0][16 + r0][16 * x + c0]));
+                const t8_h8 xh = t8_join(t8_tr(&B.x[0][r0][16 * x + c0]), t8_tr(&B.x[0][16 + r0][16 * x + c0]));
                 if (XPL == 2) {
-                    const t8_h8 xl = t8_join(t8_tr(&xi[XPL - 1][r0][16 * x + c0]), t8_tr(&xi[XPL - 1][16 + r0][16 * x + c0]));
+                    const t8_h8 xl = t8_join(t8_tr(&B.x[XPL - 1][r0][16 * x + c0]), t8_tr(&B.x[XPL - 1][16 + r0][16 * x + c0]));
 #pragma unroll
                     for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b], xl, accw[b][x], 0, 0, 0);
                 }
@@ -254,9 +318,12 @@ __global__ void __launch_bounds__(256, 2) k_tape8_linear_bwd(const T8LinArgs a) 
                 for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b], xh, accw[b][x], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
         // ---- dx = act'(v) (dz W): lane = row 16 rb + n16, features 4 q4 .. + 3 of the block
         if (a.dx) {
-            const float invG = t8_pow2(ze - 13);
+            const int e = we + ze - 280;
+            float* const bx = a.dx + row0 * a.lddx + k0;
+            const unsigned ox = ((unsigned)n16 * (unsigned)a.lddx + 16 * NBK * wave + 4 * q4) * 4u;
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb) {
                 const long r = row0 + 16 * rb + n16;
@@ -265,18 +332,22 @@ __global__ void __launch_bounds__(256, 2) k_tape8_linear_bwd(const T8LinArgs a) 
                     const int f = 16 * (NBK * wave + b) + 4 * q4, k = k0 + f;
                     t8_f4 v;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = acc[b][rb][i] * wscale * invG;
+                    for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(acc[b][rb][i], e);
                     if (ACT == ACT_RELU) {
-                        const unsigned w = ci[16 * rb + n16][f / 4];
+                        const unsigned w = B.c[16 * rb + n16][f / 4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] = (w >> (8 * i)) & 0xFFu ? v[i] : 0.f;
                     }
                     if (ACT == ACT_SWISH) {
-                        const t8_f4 x = t8_decode4<KIND>(ci[16 * rb + n16][f / 4], bi[16 * rb + n16][f / 32]);
+                        const t8_f4 x = t8_decode4<KIND>(B.c[16 * rb + n16][f / 4], B.b[16 * rb + n16][f / 32]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] *= t8_dswish(x[i]);
                     }
-                    if (r < a.M) {
+                    if (FULL) {
+                        float* o = bx + 16 * rb * a.lddx + 16 * b;
+                        T8_UNIFORM(o);
+                        if (16 * rb + n16 >= done) t8_put<t8_f4>(o, ox, v);
+                    } else if (r < a.M) {
                         float* o = a.dx + r * a.lddx + k;
                         if (a.add_dx) v += t8_load4(o, a.xvec && k < a.K, a.K - k);
                         t8_store4(o, a.xvec && k < a.K, a.K - k, v);
@@ -284,49 +355,60 @@ __global__ void __launch_bounds__(256, 2) k_tape8_linear_bwd(const T8LinArgs a) 
                 }
             }
         }
+        }
+        // ---- the stretch's part of the workgroup's sums: C/D row 4 q4 + i = feature of dz, column n16 = feature of x
+        // (the base hidden: 32 addresses would be kept in registers across the loop)
+        auto sums = [&](bool add) {
+            const unsigned ol = ((unsigned)(4 * q4) * KP + n16) * 4u;
+#pragma unroll
+            for (int b = 0; b < NBN; ++b)
+#pragma unroll
+                for (int x = 0; x < KB; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float* o = wout + (16 * (NBN * wave + b) + i) * KP + 16 * x;
+                        T8_UNIFORM(o);
+                        const float v = __builtin_amdgcn_ldexpf(accw[b][x][i], ze + xe - 272);
+                        t8_put<float>(o, ol, add ? t8_at<float>(o, ol) + v : v);
+                    }
+        };
+        if (first) sums(false);
+        else sums(true);
+        first = false;
     }
-    // ---- partial sums: C/D row 4 q4 + i = feature of dz, column n16 = feature of x
-    float* wout = a.wpart + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * NP * KP;
-    const float s0 = t8_pow2(ze - 13), s1 = t8_pow2(xe - 7);
-#pragma unroll
-    for (int b = 0; b < NBN; ++b)
-#pragma unroll
-        for (int x = 0; x < KB; ++x)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                wout[(16 * (NBN * wave + b) + 4 * q4 + i) * KP + 16 * x + n16] = accw[b][x][i] * s0 * s1;
     if (blockIdx.y == 0) {                                                    // the lanes that hold the same columns of dz, in order
-        float* s = reinterpret_cast<float*>(&zi[0][0][0]);
+        float* s = reinterpret_cast<float*>(&sb[0]);
         wg_barrier();
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[zr * NP + zc + i] = bsum[i];
         wg_barrier();
         if (tid < NP) {
             float t = 0.f;
-            for (int r = 0; r < 256 / LPR; ++r) t += s[r * NP + tid];
+            for (int r = 0; r < RPL; ++r) t += s[r * NP + tid];
             a.bpart[(size_t)blockIdx.x * NP + tid] = t;
         }
     }
 }
 
-// dW[n][k] (+)= sum over the workgroups of their partial sums, in order: a workgroup takes 64 neighbouring sums, its four waves a quarter of the
-// partials each.  blockIdx.y = block of K; the last one: db
-__global__ void __launch_bounds__(256) k_tape8_linear_sum(const float* __restrict__ wpart, const float* __restrict__ bpart, int nwg, int NP, int KP, int N, int K,
+// dW[n][k] (+)= sum over the workgroups of their partial sums, in order: a workgroup takes 64 neighbouring sums, its sixteen waves a run of the
+// partials each (short chains: the reads' latency is what this kernel takes, and the sums' rounding grows with their length).  blockIdx.y = block of K; the last one: db
+__global__ void __launch_bounds__(1024) k_tape8_linear_sum(const float* __restrict__ wpart, const float* __restrict__ bpart, int nwg, int NP, int KP, int N, int K,
                                                           float* __restrict__ dW, long lddw, float* __restrict__ db, int add) {
-    __shared__ float s[4][64];
+    __shared__ float s[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool bias = blockIdx.y == gridDim.y - 1;
     const int o = blockIdx.x * 64 + lane, n_out = bias ? NP : NP * KP;
     if (blockIdx.x * 64 >= n_out) return;
     const float* p = bias ? bpart : wpart + (size_t)blockIdx.y * nwg * NP * KP;
     float t = 0.f;
-    const int per = (nwg + 3) / 4, w1 = min(nwg, (wave + 1) * per);
+    const int per = (nwg + 15) / 16, w1 = min(nwg, (wave + 1) * per);
 #pragma unroll 8
     for (int w = wave * per; w < w1; ++w) t += p[(size_t)w * n_out + o];
     s[wave][lane] = t;
     __syncthreads();
     if (wave) return;
-    t = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
+#pragma unroll
+    for (int w = 1; w < 16; ++w) t += s[w][lane];
     const int n = bias ? o : o / KP, k = bias ? 0 : blockIdx.y * KP + o % KP;
     if (n >= N || k >= K) return;
     float* d = bias ? db + n : dW + n * lddw + k;
@@ -353,11 +435,18 @@ extern "C" int magnet_tape8_linear_bwd_workspace(long M, int N, int K, long* flo
     return 0;
 }
 
-template <int NP, int KP>
+template <int NP, int KP, bool FULL>
 static void t8_lin_launch(const T8LinArgs& a, int act, dim3 grid, hipStream_t st) {
-    if (act == ACT_RELU) k_tape8_linear_bwd<NP, KP, ACT_RELU><<<grid, 256, 0, st>>>(a);
-    else if (act == ACT_SWISH) k_tape8_linear_bwd<NP, KP, ACT_SWISH><<<grid, 256, 0, st>>>(a);
-    else k_tape8_linear_bwd<NP, KP, ACT_NONE><<<grid, 256, 0, st>>>(a);
+    if (act == ACT_RELU) k_tape8_linear_bwd<NP, KP, ACT_RELU, FULL><<<grid, T8_WAVES(NP, KP) * 64, 0, st>>>(a);
+    else if (act == ACT_SWISH) k_tape8_linear_bwd<NP, KP, ACT_SWISH, FULL><<<grid, T8_WAVES(NP, KP) * 64, 0, st>>>(a);
+    else k_tape8_linear_bwd<NP, KP, ACT_NONE, FULL><<<grid, T8_WAVES(NP, KP) * 64, 0, st>>>(a);
+}
+template <bool FULL>
+static void t8_lin_shape(const T8LinArgs& a, int np, int kp, int act, dim3 grid, hipStream_t st) {
+    if (np == 128 && kp == 128) t8_lin_launch<128, 128, FULL>(a, act, grid, st);
+    else if (np == 128) t8_lin_launch<128, 64, FULL>(a, act, grid, st);
+    else if (kp == 128) t8_lin_launch<64, 128, FULL>(a, act, grid, st);
+    else t8_lin_launch<64, 64, FULL>(a, act, grid, st);
 }
 
 extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void* codes, const void* bytes, const float* w, long ldw, long M, int N, int K,
@@ -383,11 +472,11 @@ extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void
         a.zvec = !(n & 3) && !(ldz & 3) && !((uintptr_t)a.dz & 15);
         a.xvec = !(K & 3) && !(lddx & 3) && !((uintptr_t)dx & 15);
         a.add_dx = n0 > 0;
-        if (np == 128 && kp == 128) t8_lin_launch<128, 128>(a, act, grid, st);
-        else if (np == 128) t8_lin_launch<128, 64>(a, act, grid, st);
-        else if (kp == 128) t8_lin_launch<64, 128>(a, act, grid, st);
-        else t8_lin_launch<64, 64>(a, act, grid, st);
-        k_tape8_linear_sum<<<dim3((np * kp + 63) / 64, kb + 1), 256, 0, st>>>(a.wpart, a.bpart, grid.x, np, kp, n, K, dW + n0 * lddw, lddw, db ? db + n0 : nullptr, accumulate);
+        // (32-bit byte offsets inside a step of 32 rows)
+        const bool full = M >= 32 && N == np && !(K % kp) && a.zvec && (a.xvec || !dx) && ldz < (1l << 24) && lddx < (1l << 24) && ldw < (1l << 24);
+        if (full) t8_lin_shape<true>(a, np, kp, act, grid, st);
+        else t8_lin_shape<false>(a, np, kp, act, grid, st);
+        k_tape8_linear_sum<<<dim3((np * kp + 63) / 64, kb + 1), 1024, 0, st>>>(a.wpart, a.bpart, grid.x, np, kp, n, K, dW + n0 * lddw, lddw, db ? db + n0 : nullptr, accumulate);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
     }
