@@ -556,7 +556,7 @@ int magnet_tape8_unpack(const void* codes, const void* bytes, long M, int W, int
  *   dx [M][K] = act'(v) (dz W),  dW [N][K] (+)= dz^T x,  db [N] (+)= column sums of dz       (dx, db may be NULL)
  * act: MAGNET_ACT_NONE (signed tape of x), _RELU (relu tape of x: act' = x > 0), _SWISH (signed tape of Swish's argument).  dx must not
  * overlap dz.  M = 0 zeroes dW / db (accumulate == 0).  workspace: magnet_tape8_linear_bwd_workspace(M, N, K) floats. */
-int magnet_tape8_linear_bwd_workspace(long M, int N, int K, long* floats);
+int magnet_tape8_linear_bwd_workspace(long M, long N, long K, long* floats);
 int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void* codes, const void* bytes, const float* w, long ldw, long M, int N, int K,
                                 int act, float* dx, long lddx, float* dW, long lddw, float* db, int accumulate, float* workspace,
                                 void* stream);
@@ -574,7 +574,7 @@ int magnet_norm_join(const void* x, long ldx, const void* f, long ldf, int dtype
 /* Its backward from gy = d y, gh = d h (pre norm only) and the tapes: dx, df [M][W], dgate [G][W] (dtype), d_scale / d_post_g / d_post_b /
  * d_pre_g / d_pre_b [W] (fp32, written; NULL: not wanted).  M >= 1.  workspace: magnet_norm_join_bwd_workspace(M, W, G or 0) floats.  The sums
  * over rows are added in a fixed order. */
-int magnet_norm_join_bwd_workspace(long M, int W, long G, long* floats);
+int magnet_norm_join_bwd_workspace(long M, long W, long G, long* floats);
 int magnet_norm_join_bwd(const void* gy, long ldgy, const void* gh, long ldgh, int dtype, long M, int W, int layer, const float* post_g,
                          const float* post_b, const float* pre_g, const float* pre_b, const void* gate, long ldg, long G, const float* scale_v,
                          float scale, const void* post_codes, const void* post_bytes, const float* post_rstd, const void* pre_codes,

@@ -447,10 +447,10 @@ static long nj_bwd_grid(long M, int W, long G, int* per_group) {
     *per_group = (int)(each < n ? each : n);
     return G * *per_group;
 }
-extern "C" int magnet_norm_join_bwd_workspace(long M, int W, long G, long* floats) {
+extern "C" int magnet_norm_join_bwd_workspace(long M, long W, long G, long* floats) {
     int per = 0;
     if (M < 1 || W < 1 || W > NJ_MAX_W || G < 0 || (G && M % G)) return -2;
-    *floats = nj_bwd_grid(M, W, G, &per) * 4 * W;
+    *floats = nj_bwd_grid(M, (int)W, G, &per) * 4 * W;
     return 0;
 }
 

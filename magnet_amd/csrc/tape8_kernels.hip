@@ -1,13 +1,14 @@
 // Writing and reading the 8-bit tape (the format: tape8.cuh).
 //
 // Both kernels are one pass bound by HBM: a pack reads the row (4 / 2 bytes a value) and writes 33/32 bytes a value, an unpack the other
-// way.  A lane takes four neighbouring columns, eight neighbouring lanes one block of 32: the block's top is three lane exchanges, the
-// codes leave as one word per lane, a wave's stores are whole lines.  A lane walks its positions by adding the grid's stride, split once
-// into rows and columns: no division in the loop, and 64-bit row offsets.
+// way.  Packing, a lane takes eight neighbouring columns, four neighbouring lanes one block of 32: the block's top is two lane permutes, the
+// codes leave as eight bytes per lane, a wave's stores are whole lines.  A lane walks its positions by adding the grid's stride, split once into
+// rows and columns: no division in the loop, and 64-bit row offsets.
 #include "common.cuh"
 #include "tape8.cuh"
 
-struct T8Walk {                          // position (row, group of four columns) of a flat index, and the step between two visits
+#define T8_CPL 8                         // columns per lane of a pack
+struct T8Walk {                          // position (row, group of columns) of a flat index, and the step between two visits
     long row, drow;
     int g, dg, G;
     __device__ __forceinline__ T8Walk(long i, long stride, int groups) {
@@ -24,32 +25,43 @@ struct T8Walk {                          // position (row, group of four columns
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256) k_tape8_pack(const T* __restrict__ x, long ldx, long M, int W, int vec, unsigned char* __restrict__ codes,
                                                     unsigned char* __restrict__ bytes) {
-    const int groups = ((W + 31) / 32) * 8;
-    T8Walk at((long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, groups);
-    for (; at.row < M; at.next()) {      // (the eight lanes of a block leave together: groups and the stride are multiples of 8)
-        const int c = 4 * at.g;
-        const t8_f4 v = t8_load4(x + at.row * ldx + c, vec && c < W, W - c);
-        const unsigned byte = t8_byte<KIND>(t8_max8(t8_top4<KIND>(v)));
-        *reinterpret_cast<unsigned*>(codes + at.row * (4 * groups) + c) = t8_code4<KIND>(v, byte);
-        if (!(at.g & 7)) bytes[at.row * (groups / 8) + (at.g >> 3)] = (unsigned char)byte;
+    const int blocks = (W + 31) / 32;
+    T8Walk at((long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, blocks * (32 / T8_CPL));
+    for (; at.row < M; at.next()) {      // (the lanes of a block leave together: groups and the stride are multiples of 4)
+        const int c = T8_CPL * at.g;
+        t8_f4 v[T8_CPL / 4];
+        unsigned top = 0;
+#pragma unroll
+        for (int h = 0; h < T8_CPL / 4; ++h) {
+            const int ch = c + 4 * h;
+            v[h] = t8_load4(x + at.row * ldx + ch, vec && ch < W, W - ch);
+            top = max(top, t8_top4<KIND>(v[h]));
+        }
+        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));      // quad_perm 1 0 3 2, 2 3 0 1
+        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));
+        const unsigned byte = t8_byte<KIND>(top);
+        *reinterpret_cast<t8_u2*>(codes + at.row * (32 * blocks) + c) = t8_u2{t8_code4<KIND>(v[0], byte), t8_code4<KIND>(v[1], byte)};
+        if (!(at.g & 3)) bytes[at.row * blocks + (at.g >> 2)] = (unsigned char)byte;
     }
 }
 
+// (four columns per lane here: what it writes is four times what it reads, and a store instruction then covers a run of whole lines)
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256) k_tape8_unpack(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ bytes, long M, int W,
                                                       T* __restrict__ y, long ldy, int vec) {
-    const int groups = ((W + 31) / 32) * 8;
-    T8Walk at((long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, groups);
+    const int blocks = (W + 31) / 32;
+    T8Walk at((long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, blocks * 8);
     for (; at.row < M; at.next()) {
         const int c = 4 * at.g;
-        const unsigned w = *reinterpret_cast<const unsigned*>(codes + at.row * (4 * groups) + c);
-        t8_store4(y + at.row * ldy + c, vec && c < W, W - c, t8_decode4<KIND>(w, bytes[at.row * (groups / 8) + (at.g >> 3)]));
+        const unsigned w = *reinterpret_cast<const unsigned*>(codes + at.row * (32 * blocks) + c);
+        t8_store4(y + at.row * ldy + c, vec && c < W, W - c, t8_decode4<KIND>(w, bytes[at.row * blocks + (at.g >> 3)]));
     }
 }
 
-static unsigned t8_grid(long M, int W) {
-    const long n = (M * (((W + 31) / 32) * 8) + 255) / 256;
-    return (unsigned)(n < 1 ? 1 : n > 8192 ? 8192 : n);
+// one pass of every lane, up to the largest grid: a fixed number of workgroups that walk the array was 10 % slower at 2 097 152 x 128
+static unsigned t8_grid(long M, int W, int lanes_per_block) {
+    const long n = (M * ((W + 31) / 32) * lanes_per_block + 255) / 256;
+    return (unsigned)(n < 1 ? 1 : n > (1l << 24) ? 1l << 24 : n);
 }
 // four values at once: the width, the row stride and the address are multiples of four values
 static int t8_vec(const void* p, long ld, int W, size_t size) { return !(W & 3) && !(ld & 3) && !((uintptr_t)p & (4 * size - 1)); }
@@ -57,7 +69,7 @@ static int t8_vec(const void* p, long ld, int W, size_t size) { return !(W & 3) 
 template <typename T>
 static int t8_pack_as(const void* x, long ldx, long M, int W, int kind, void* codes, void* bytes, hipStream_t st) {
     const int vec = t8_vec(x, ldx, W, sizeof(T));
-    const dim3 grid(t8_grid(M, W));
+    const dim3 grid(t8_grid(M, W, 32 / T8_CPL));
     if (kind == T8_RELU)
         k_tape8_pack<T, T8_RELU><<<grid, 256, 0, st>>>((const T*)x, ldx, M, W, vec, (unsigned char*)codes, (unsigned char*)bytes);
     else
@@ -67,7 +79,7 @@ static int t8_pack_as(const void* x, long ldx, long M, int W, int kind, void* co
 template <typename T>
 static int t8_unpack_as(const void* codes, const void* bytes, long M, int W, int kind, void* y, long ldy, hipStream_t st) {
     const int vec = t8_vec(y, ldy, W, sizeof(T));
-    const dim3 grid(t8_grid(M, W));
+    const dim3 grid(t8_grid(M, W, 8));
     if (kind == T8_RELU)
         k_tape8_unpack<T, T8_RELU><<<grid, 256, 0, st>>>((const unsigned char*)codes, (const unsigned char*)bytes, M, W, (T*)y, ldy, vec);
     else

@@ -4,11 +4,11 @@
 // What has to move is dz in, dx out and 33/32 bytes a value of the tape: 1156 bytes a row at N = K = 128, where fp32 activations make it
 // 1536 (linear_bwd.hip).
 //
-// A workgroup of four waves takes steps of 32 rows of one block of at most 128 x 128 of W.  dz is split once into two fp16 planes
+// A workgroup of four waves takes steps of 32 or 64 rows of one block of at most 128 x 128 of W.  dz is split once into two fp16 planes
 // (h + l, 22 bits), the tape's codes need one plane - a code has 8 bits, fp16 holds code times a power of two exactly - (two behind
 // Swish), and both meet as 16 x 16 x 32 matrix products through LDS:
 //   dx^T = W^T dz^T   A = the wave's features of W^T, two planes kept in registers; B = rows of the dz image; products hh + hl + lh
-//   dW   = dz^T x     A, B = transposed LDS reads of the two images, k = the step's 32 rows; products (h + l) x
+//   dW   = dz^T x     A, B = transposed LDS reads of the two images, k = 32 of the step's rows; products (h + l) x
 // The error of both is a few 2^-22 of the operands' magnitude, sums are held in fp32, and the workgroups' partial sums of dW and db are added
 // in their order by a second kernel: the same bits every time.
 //
@@ -53,26 +53,24 @@ __device__ __forceinline__ float t8_sigmoid(float v, float& e) {
     e = __expf(fminf(-v, 87.0f));
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
-__device__ __forceinline__ float t8_swish(float v) {
+// Swish v s and its derivative s (1 + v (1 - s)) with 1 - s = e^-v s: no cancellation where s is near 1
+__device__ __forceinline__ float t8_swish(float v, float& d) {
     float e;
-    return v * t8_sigmoid(v, e);
-}
-// Swish's derivative s (1 + v (1 - s)) with 1 - s = e^-v s: no cancellation where s is near 1
-__device__ __forceinline__ float t8_dswish(float v) {
-    float e;
-    const float s = t8_sigmoid(v, e);
-    return s + v * s * (e * s);
+    const float s = t8_sigmoid(v, e), y = v * s;
+    d = s + y * (e * s);
+    return y;
 }
 
 #define T8_WAVES(NP, KP) ((NP) == 128 && (KP) == 128 ? 8 : 4)
+#define T8_ROWS(NP, KP, ACT) ((ACT) != ACT_SWISH ? 64 : 32)      // rows of a step
 #define T8_ZROOM 3                       // binades of dz and of the tape's bytes that may still come before the scale has to change
 #define T8_XROOM 2
-template <int NP, int KP, int XPL>
-struct T8Step {                          // a step of 32 rows in LDS; row strides of 16 halfwords more than a power of two spread the rows over the banks
-    unsigned short z[2][32][NP + 16];
-    unsigned short x[XPL][32][KP + 16];
-    unsigned c[32][KP / 4 + 4];          // the codes (the mask; Swish's argument)
-    unsigned char b[32][KP / 32];
+template <int NP, int KP, int XPL, int R, int ACT>
+struct T8Step {                          // a step of R rows in LDS; row strides of 16 halfwords more than a power of two spread the rows over the banks
+    unsigned short z[2][R][NP + 16];
+    unsigned short x[XPL][R][KP + 16];
+    unsigned c[ACT == ACT_RELU ? R : 1][KP / 4 + 4];       // the codes (the mask of dx)
+    float d[ACT == ACT_SWISH ? R : 1][KP + 4];             // Swish's derivative: formed where Swish is, from the same exponential
 };
 
 // a value at a wave-uniform base plus the lane's offset in bytes (global_* with a scalar base: the caller hides the base behind an asm statement,
@@ -92,16 +90,17 @@ __device__ __forceinline__ void t8_put(void* base, unsigned off, const V& v) {
 // A workgroup of NP and KP at most 64 has four waves, else eight: a wave owns one block of 16 features of either side (of 64 features on
 // one side, every other wave the rows' other half).
 template <int NP, int KP, int ACT, bool FULL>
-__global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ? 4 : 2) k_tape8_linear_bwd(const T8LinArgs a) {
+__global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(const T8LinArgs a) {
     constexpr int KIND = ACT == ACT_RELU ? T8_RELU : T8_SIGNED;
     constexpr int XPL = ACT == ACT_SWISH ? 2 : 1;                             // planes of x
-    constexpr int NBUF = XPL == 2 && NP == 128 && KP == 128 ? 1 : 2;          // (two such steps for two workgroups a CU are more than 160 KB)
+    constexpr int R = T8_ROWS(NP, KP, ACT);
+    typedef T8Step<NP, KP, XPL, R, ACT> Step;
     constexpr int NW = T8_WAVES(NP, KP), LANES = 64 * NW;
-    constexpr int LPR = NP / 4, RPL = LANES / LPR, NLD = 32 / RPL;            // lanes per row of dz, rows per pass, passes
-    constexpr int CPT = 32 * KP / LANES, CPR = KP / CPT, CW = CPT / 4;        // codes per lane (8 or 16), lanes per row, words
+    constexpr int LPR = NP / 4, RPL = LANES / LPR, NLD = R / RPL;             // lanes per row of dz, rows per pass, passes
+    constexpr int CPT = R * KP / LANES, CPR = KP / CPT, CW = CPT / 4;        // codes per lane (8 or 16), lanes per row, words
     constexpr int NBK = KP / 16 / NW, NBN = NP / 16 / NW, NT = NP / 32, KB = KP / 16;   // a wave's blocks of 16 features of x / of dz
     typedef unsigned t8_cw __attribute__((ext_vector_type(CW)));
-    __shared__ __attribute__((aligned(16))) T8Step<NP, KP, XPL> sb[NBUF];
+    __shared__ __attribute__((aligned(16))) Step sb[2];
     __shared__ unsigned red[NW], flag[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
@@ -114,10 +113,10 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ?
     t8_f4 dv[NLD];
     t8_cw cv = t8_cw(0u);
     unsigned bv = 0;
-    int shift = 0;                                                            // FULL, the last step: it takes the last 32 rows, this many of them done
+    int shift = 0;                                                            // FULL, the last step: it takes the last R rows, this many of them done
     auto load = [&](long step) {
         if (FULL) {
-            const long row = min(step * 32, a.M - 32);
+            const long row = min(step * R, a.M - R);
             const unsigned oz = ((unsigned)zr * (unsigned)a.ldz + zc) * 4u, oc = (unsigned)cr * (unsigned)a.ldc + cc, ob = (unsigned)cr * (unsigned)lb + cc / 32;
             const unsigned char *bc = a.codes + row * a.ldc + k0, *bb = a.bytes + row * lb + k0 / 32;
             T8_UNIFORM(bc);
@@ -133,15 +132,15 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ?
         }
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
-            const long r = step * 32 + zr + i * RPL;
+            const long r = step * R + zr + i * RPL;
             dv[i] = r < a.M ? t8_load4(a.dz + r * a.ldz + zc, a.zvec && zc < a.N, a.N - zc) : t8_f4{0.f, 0.f, 0.f, 0.f};
         }
-        const long r = step * 32 + cr;
+        const long r = step * R + cr;
         const bool on = c_on && r < a.M;
         cv = on ? *reinterpret_cast<const t8_cw*>(a.codes + r * a.ldc + k0 + cc) : t8_cw(0u);
         bv = on ? a.bytes[r * lb + (k0 + cc) / 32] : 0u;
     };
-    const long nsteps = (a.M + 31) / 32;
+    const long nsteps = (a.M + R - 1) / R;
     long step = blockIdx.x;
     load(step);
     // ---- the wave's features of W^T: A operands (lane = feature of x, register j of k group q4 = feature 32 t + 8 q4 + j of dz)
@@ -185,7 +184,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ?
     t8_f4 bsum = {0.f, 0.f, 0.f, 0.f};
     int ze = 14, xe = 8;                                                      // bounds: dz is staged times 2^(140 - ze), codes times 2^(byte - xe + 5)
     // ---- this lane's part of the step in its two images; true if something lies above the bounds
-    auto stage = [&](T8Step<NP, KP, XPL>& B) -> bool {
+    auto stage = [&](Step& B) -> bool {
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
@@ -207,8 +206,16 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ?
 #pragma unroll
             for (int j = 0; j < CW; ++j) {
                 const t8_f4 v = t8_decode4<KIND>(cv[j], bv);
-                split_f16_prod(t8_swish(v[0]), up, t8_swish(v[1]), up, p[0][2 * j], p[XPL - 1][2 * j]);
-                split_f16_prod(t8_swish(v[2]), up, t8_swish(v[3]), up, p[0][2 * j + 1], p[XPL - 1][2 * j + 1]);
+                t8_f4 y, dy;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float d;
+                    y[i] = t8_swish(v[i], d);
+                    dy[i] = d;
+                }
+                split_f16_prod(y[0], up, y[1], up, p[0][2 * j], p[XPL - 1][2 * j]);
+                split_f16_prod(y[2], up, y[3], up, p[0][2 * j + 1], p[XPL - 1][2 * j + 1]);
+                *reinterpret_cast<t8_f4*>(&B.d[cr][cc + 4 * j]) = dy;
             }
         } else {
             // byte c beside 0x64 is the fp16 number 1024 + c (signed: c + 128 after the sign bit is turned): times the power of two, less what it
@@ -228,8 +235,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ?
 #pragma unroll
             for (int j = 0; j < CPT / 8; ++j)
                 *reinterpret_cast<t8_u4*>(&B.x[q][cr][cc + 8 * j]) = t8_u4{p[q][4 * j], p[q][4 * j + 1], p[q][4 * j + 2], p[q][4 * j + 3]};
-        if (ACT != ACT_NONE) *reinterpret_cast<t8_cw*>(&B.c[cr][cc / 4]) = cv;
-        if (ACT == ACT_SWISH && !(cc & 31)) B.b[cr][cc / 32] = (unsigned char)bv;
+        if (ACT == ACT_RELU) *reinterpret_cast<t8_cw*>(&B.c[cr][cc / 4]) = cv;
         return m >= t8_pow2(ze + 1) || (!bad && (int)bv > xe);
     };
     float* const wout = a.wpart + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * NP * KP;
@@ -261,9 +267,8 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ?
             for (int x = 0; x < KB; ++x) accw[b][x] = f32x4{0.f, 0.f, 0.f, 0.f};
         // (a stretch's first step is what its bounds were made of: nothing to ask - and what is not finite would ask for more for ever)
         for (bool fresh = true; step < nsteps; step += gridDim.x, ++it, fresh = false) {
-        T8Step<NP, KP, XPL>& B = sb[it & (NBUF - 1)];
-        if (NBUF == 1 && !fresh) wg_barrier();                                // the step before has been read
-        if (FULL) shift = (int)(step * 32 - min(step * 32, a.M - 32));
+        Step& B = sb[it & 1];
+        if (FULL) shift = (int)(step * R - min(step * R, a.M - R));
         const bool over = stage(B);
         if (!fresh && __any(over) && lane == 0) flag[it & 1] = 1u;
         wg_barrier();
@@ -271,32 +276,69 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ?
 #pragma unroll
         for (int i = 0; i < NLD; ++i)
             if (!FULL || zr + i * RPL >= shift) bsum += dv[i];
-        const long row0 = FULL ? min(step * 32, a.M - 32) : step * 32;
+        const long row0 = FULL ? min(step * R, a.M - R) : step * R;
         const int done = shift;
         asm volatile("" ::: "memory");
         load(min(step + (long)gridDim.x, nsteps - 1));                        // (past the last step: rows that nobody uses)
         asm volatile("" ::: "memory");
-        // ---- dx^T: acc[b][rb] = features 16 (NBK wave + b) .. of rows 16 rb ..
-        f32x4 acc[NBK][2];
+        // ---- dx, 32 rows at a time: dx^T, acc[b][rb] = features 16 (NBK wave + b) .. of rows 16 rb ..
 #pragma unroll
-        for (int b = 0; b < NBK; ++b) acc[b][0] = acc[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int r32 = 0; r32 < R; r32 += 32) {
+            f32x4 acc[NBK][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+            for (int b = 0; b < NBK; ++b) acc[b][0] = acc[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                const t8_h8 zh = *reinterpret_cast<const t8_h8*>(&B.z[0][16 * rb + n16][32 * t + 8 * q4]);
-                const t8_h8 zl = *reinterpret_cast<const t8_h8*>(&B.z[1][16 * rb + n16][32 * t + 8 * q4]);
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl[b][t], zh, acc[b][rb], 0, 0, 0);
+                for (int rb = 0; rb < 2; ++rb) {
+                    const t8_h8 zh = *reinterpret_cast<const t8_h8*>(&B.z[0][r32 + 16 * rb + n16][32 * t + 8 * q4]);
+                    const t8_h8 zl = *reinterpret_cast<const t8_h8*>(&B.z[1][r32 + 16 * rb + n16][32 * t + 8 * q4]);
 #pragma unroll
-                for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zl, acc[b][rb], 0, 0, 0);
+                    for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl[b][t], zh, acc[b][rb], 0, 0, 0);
 #pragma unroll
-                for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zh, acc[b][rb], 0, 0, 0);
+                    for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zl, acc[b][rb], 0, 0, 0);
+#pragma unroll
+                    for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zh, acc[b][rb], 0, 0, 0);
+                }
+            __builtin_amdgcn_sched_barrier(0);                                // (without these the reads of all parts move up and the registers run out)
+            // dx = act'(v) (dz W): lane = row 16 rb + n16, features 4 q4 .. + 3 of the block
+            if (a.dx) {
+                const int e = we + ze - 280;
+                float* const bx = a.dx + (row0 + r32) * a.lddx + k0;
+                const unsigned ox = ((unsigned)n16 * (unsigned)a.lddx + 16 * NBK * wave + 4 * q4) * 4u;
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb) {
+                    const int lr = r32 + 16 * rb + n16;                       // row of the step
+#pragma unroll
+                    for (int b = 0; b < NBK; ++b) {
+                        const int f = 16 * (NBK * wave + b) + 4 * q4, k = k0 + f;
+                        t8_f4 v;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(acc[b][rb][i], e);
+                        if (ACT == ACT_RELU) {
+                            const unsigned w = B.c[lr][f / 4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] = (w >> (8 * i)) & 0xFFu ? v[i] : 0.f;
+                        }
+                        if (ACT == ACT_SWISH) v *= *reinterpret_cast<const t8_f4*>(&B.d[lr][f]);
+                        if (FULL) {
+                            float* o = bx + 16 * rb * a.lddx + 16 * b;
+                            T8_UNIFORM(o);
+                            if (lr >= done) t8_put<t8_f4>(o, ox, v);
+                        } else if (row0 + lr < a.M) {
+                            float* o = a.dx + (row0 + lr) * a.lddx + k;
+                            if (a.add_dx) v += t8_load4(o, a.xvec && k < a.K, a.K - k);
+                            t8_store4(o, a.xvec && k < a.K, a.K - k, v);
+                        }
+                    }
+                }
             }
-        __builtin_amdgcn_sched_barrier(0);                                    // (without these the reads of all three parts move up and the registers run out)
-        // ---- dW += dz^T x over the step's rows (k group q4: rows 4 q4 .. + 3 and 16 + 4 q4 .. + 3 of both operands)
-        {
-            const int r0 = 4 * q4 + (n16 >> 2), c0 = 4 * (n16 & 3);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // ---- dW += dz^T x, 32 rows at a time (k group q4: rows 4 q4 .. + 3 and 16 + 4 q4 .. + 3 of both operands)
+#pragma unroll
+        for (int r32 = 0; r32 < R; r32 += 32) {
+            const int r0 = r32 + 4 * q4 + (n16 >> 2), c0 = 4 * (n16 & 3);
             t8_h8 ah[NBN], al[NBN];
 #pragma unroll
             for (int b = 0; b < NBN; ++b) {
@@ -316,43 +358,6 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, T8_WAVES(NP, KP) == 8 ?
                 for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[b], xh, accw[b][x], 0, 0, 0);
 #pragma unroll
                 for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b], xh, accw[b][x], 0, 0, 0);
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        // ---- dx = act'(v) (dz W): lane = row 16 rb + n16, features 4 q4 .. + 3 of the block
-        if (a.dx) {
-            const int e = we + ze - 280;
-            float* const bx = a.dx + row0 * a.lddx + k0;
-            const unsigned ox = ((unsigned)n16 * (unsigned)a.lddx + 16 * NBK * wave + 4 * q4) * 4u;
-#pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                const long r = row0 + 16 * rb + n16;
-#pragma unroll
-                for (int b = 0; b < NBK; ++b) {
-                    const int f = 16 * (NBK * wave + b) + 4 * q4, k = k0 + f;
-                    t8_f4 v;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(acc[b][rb][i], e);
-                    if (ACT == ACT_RELU) {
-                        const unsigned w = B.c[16 * rb + n16][f / 4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = (w >> (8 * i)) & 0xFFu ? v[i] : 0.f;
-                    }
-                    if (ACT == ACT_SWISH) {
-                        const t8_f4 x = t8_decode4<KIND>(B.c[16 * rb + n16][f / 4], B.b[16 * rb + n16][f / 32]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] *= t8_dswish(x[i]);
-                    }
-                    if (FULL) {
-                        float* o = bx + 16 * rb * a.lddx + 16 * b;
-                        T8_UNIFORM(o);
-                        if (16 * rb + n16 >= done) t8_put<t8_f4>(o, ox, v);
-                    } else if (r < a.M) {
-                        float* o = a.dx + r * a.lddx + k;
-                        if (a.add_dx) v += t8_load4(o, a.xvec && k < a.K, a.K - k);
-                        t8_store4(o, a.xvec && k < a.K, a.K - k, v);
-                    }
-                }
             }
         }
         }
@@ -423,15 +428,17 @@ __global__ void __launch_bounds__(256) k_tape8_fill0(float* __restrict__ p, long
 
 #define T8_BLOCK 128
 static int t8_pad(int n) { return n <= 64 ? 64 : 128; }                       // a block of at most 128 features, as 64 or 128
-static int t8_lin_grid(long M, int kblocks) {
-    const long steps = (M + 31) / 32, most = 512 / (kblocks < 4 ? kblocks : 4);
+// one workgroup a CU of eight waves, two (three) of four; fewer where K has several blocks
+static int t8_lin_grid(long M, int np, int kp, int kblocks, int act) {
+    const int R = T8_ROWS(np, kp, act);
+    const long steps = (M + R - 1) / R, most = (np == 128 && kp == 128 ? 256 : 512) / (kblocks < 4 ? kblocks : 4);
     return (int)(steps < most ? steps : most);
 }
 
-extern "C" int magnet_tape8_linear_bwd_workspace(long M, int N, int K, long* floats) {
-    if (M < 0 || N < 1 || K < 1) return -2;
-    const int kp = t8_pad(K), kb = (K + kp - 1) / kp, np = t8_pad(N);
-    *floats = (long)t8_lin_grid(M, kb) * ((long)np * kp * kb + np);
+extern "C" int magnet_tape8_linear_bwd_workspace(long M, long N, long K, long* floats) {
+    if (M < 0 || N < 1 || K < 1 || N > INT32_MAX || K > INT32_MAX) return -2;
+    const int kp = t8_pad((int)K), kb = (int)((K + kp - 1) / kp), np = t8_pad((int)N);
+    *floats = (long)t8_lin_grid(M, np, kp, kb, ACT_SWISH) * ((long)np * kp * kb + np);      // (most workgroups: steps of 32 rows)
     return 0;
 }
 
@@ -462,9 +469,10 @@ extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void
         return (int)hipGetLastError();
     }
     const int kp = t8_pad(K), kb = (K + kp - 1) / kp;
-    const dim3 grid(t8_lin_grid(M, kb), kb);
+    const int np = t8_pad(N);
+    const dim3 grid(t8_lin_grid(M, np, kp, kb, act), kb);
     for (int n0 = 0; n0 < N; n0 += T8_BLOCK) {
-        const int n = N - n0 < T8_BLOCK ? N - n0 : T8_BLOCK, np = t8_pad(N);
+        const int n = N - n0 < T8_BLOCK ? N - n0 : T8_BLOCK;
         T8LinArgs a;
         a.dz = dz + n0, a.codes = (const unsigned char*)codes, a.bytes = (const unsigned char*)bytes, a.w = w + n0 * ldw, a.dx = dx;
         a.wpart = workspace, a.bpart = workspace + (size_t)grid.x * np * kp * kb;
@@ -473,7 +481,7 @@ extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void
         a.xvec = !(K & 3) && !(lddx & 3) && !((uintptr_t)dx & 15);
         a.add_dx = n0 > 0;
         // (32-bit byte offsets inside a step of 32 rows)
-        const bool full = M >= 32 && N == np && !(K % kp) && a.zvec && (a.xvec || !dx) && ldz < (1l << 24) && lddx < (1l << 24) && ldw < (1l << 24);
+        const bool full = M >= 64 && N == np && !(K % kp) && a.zvec && (a.xvec || !dx) && ldz < (1l << 24) && lddx < (1l << 24) && ldw < (1l << 24);
         if (full) t8_lin_shape<true>(a, np, kp, act, grid, st);
         else t8_lin_shape<false>(a, np, kp, act, grid, st);
         k_tape8_linear_sum<<<dim3((np * kp + 63) / 64, kb + 1), 1024, 0, st>>>(a.wpart, a.bpart, grid.x, np, kp, n, K, dW + n0 * lddw, lddw, db ? db + n0 : nullptr, accumulate);

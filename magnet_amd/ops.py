@@ -836,26 +836,34 @@ def _is_tensor(t, name):
         raise TypeError(f"magnet_amd: {name} must be a tensor (got {type(t).__name__})")
 
 
-def _on_device(**tensors):
+def _on_device(*tensors):
     """every tensor that is there lives on the current HIP device (checked last: a call that is wrong anyway says so on any machine)"""
-    for name, t in tensors.items():
+    cur = -1
+    for t in tensors:
         for u in ((t.codes, t.bytes) if isinstance(t, Tape8) else (t,)):
             if u is None:
                 continue
             if not u.is_cuda:
-                raise RuntimeError(f"magnet_amd: {name} must live on a HIP device (got {u.device}); there is no CPU path")
-            _same_device(u, name)
+                raise RuntimeError(f"magnet_amd: a tensor must live on a HIP device (got {u.device}); there is no CPU path")
+            if cur < 0:
+                cur = _cur_dev()
+            if u.get_device() != cur:
+                _same_device(u, "a tensor")
 
 
 def _matrix(t, name, dtypes, shape=None):
     """a 2-D tensor of one of ``dtypes`` whose rows are runs of neighbouring values (copied where they are not)"""
-    _is_tensor(t, name)
+    if not isinstance(t, torch.Tensor):
+        _is_tensor(t, name)
     if t.dtype not in dtypes:
         raise TypeError(f"magnet_amd: {name} is {t.dtype}; supported: {', '.join(str(d) for d in dtypes)}")
-    if t.dim() != 2 or t.shape[1] < 1 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"magnet_amd: {name} has shape {tuple(t.shape)}" + (f", expected {tuple(shape)}" if shape is not None else ", expected [rows, width >= 1]"))
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
+    s = tuple(t.shape)
+    if len(s) != 2 or s[1] < 1 or (shape is not None and s != shape):
+        raise ValueError(f"magnet_amd: {name} has shape {s}" + (f", expected {shape}" if shape is not None else ", expected [rows, width >= 1]"))
+    if not t.is_contiguous():
+        st = t.stride()
+        if (st[1] != 1 and s[1] > 1) or (s[0] > 1 and st[0] < s[1]):
+            t = t.contiguous()
     return t
 
 
@@ -891,7 +899,7 @@ def tape8_pack(x, kind="signed", out=None) -> Tape8:
     x = _matrix(x, "x", tuple(_T8_DTYPES))
     M, W = x.shape
     t = _tape8_ok(out, "out", kind, W, M) if out is not None else None
-    _on_device(x=x, out=t)
+    _on_device(x, t)
     if t is None:
         t = tape8_empty(M, W, kind, x.device)
     L.check(L.lib().magnet_tape8_pack(_p(x), _T8_DTYPES[x.dtype], _ld(x), C.c_long(M), W, TAPE8_KINDS[kind], _p(t.codes), _p(t.bytes), _stream()), "tape8_pack")
@@ -903,18 +911,28 @@ def tape8_unpack(t: Tape8, dtype=torch.float32, out=None):
     _tape8_ok(t)
     if dtype not in _T8_DTYPES:
         raise TypeError(f"magnet_amd: a tape is read as {', '.join(str(d) for d in _T8_DTYPES)} (got {dtype})")
-    _on_device(tape=t)
+    _on_device(t)
     y = _out_matrix(out, "out", dtype, (t.rows, t.width), t.codes.device)
-    _on_device(out=y)
+    _on_device(y)
     L.check(L.lib().magnet_tape8_unpack(_p(t.codes), _p(t.bytes), C.c_long(t.rows), t.width, TAPE8_KINDS[t.kind], _p(y), _T8_DTYPES[dtype], _ld(y), _stream()),
             "tape8_unpack")
     return y
 
 
+_FLOATS: dict = {}
+
+
 def _floats(entry, *args):
-    n = C.c_long(0)
-    L.check(getattr(L.lib(), entry)(*args, C.byref(n)), entry)
-    return n.value
+    """size of a workspace: a pure function of the sizes, asked once"""
+    key = (entry, args)
+    n = _FLOATS.get(key)
+    if n is None:
+        out = C.c_long(0)
+        L.check(getattr(L.lib(), entry)(*(C.c_long(a) for a in args), C.byref(out)), entry)
+        if len(_FLOATS) >= 4096:
+            _FLOATS.clear()
+        n = _FLOATS[key] = max(out.value, 1)
+    return n
 
 
 def tape8_linear_bwd(dz, tape: Tape8, w, act="none", *, need_dx=True, dx=None, dW=None, db=None, accumulate=False):
@@ -936,13 +954,13 @@ def tape8_linear_bwd(dz, tape: Tape8, w, act="none", *, need_dx=True, dx=None, d
     for o, name, shape in ((dx, "dx", (M, K)), (dW, "dW", (N, K)), (db, "db", (N,))):
         if o is not None and _overlap(_out_matrix(o, name, torch.float32, shape, None), dz):
             raise ValueError(f"magnet_amd: {name} must not overlap dz")
-    _on_device(dz=dz, tape=tape, w=w, dx=dx, dW=dW, db=db)
+    _on_device(dz, tape, w, dx, dW, db)
     dev = dz.device
     if need_dx and dx is None:
         dx = torch.empty(M, K, dtype=torch.float32, device=dev)
     dW = torch.empty(N, K, dtype=torch.float32, device=dev) if dW is None else dW
     db = torch.empty(N, dtype=torch.float32, device=dev) if db is None else db
-    ws = torch.empty(max(_floats("magnet_tape8_linear_bwd_workspace", C.c_long(M), N, K), 1), device=dev, dtype=torch.float32)
+    ws = torch.empty(_floats("magnet_tape8_linear_bwd_workspace", M, N, K), device=dev, dtype=torch.float32)
     L.check(L.lib().magnet_tape8_linear_bwd_f32(_p(dz), _ld(dz), _p(tape.codes), _p(tape.bytes), _p(w), _ld(w), C.c_long(M), N, K, _T8_ACTS[act],
                                                 _p(dx), _ld(dx) if dx is not None else C.c_long(0), _p(dW), _ld(dW), _p(db), int(bool(accumulate)), _p(ws),
                                                 _stream()), "tape8_linear_bwd")
@@ -1020,7 +1038,7 @@ def norm_join(x, f, *, post=None, pre=None, gate=None, scale=1.0, norm="layer", 
     x, (pg, pb), (qg, qb), gate, G, sv, sc = _join_args(x, "x", post, pre, gate, scale, norm)
     M, W = x.shape
     f = _matrix(f, "f", (x.dtype,), (M, W))
-    _on_device(x=x, f=f, post=pg, post_bias=pb, pre=qg, pre_bias=qb, gate=gate, scale=sv)
+    _on_device(x, f, pg, pb, qg, qb, gate, sv)
     dev = x.device
     r = NormJoin(torch.empty(M, W, dtype=x.dtype, device=dev), torch.empty(M, W, dtype=x.dtype, device=dev) if qg is not None else None)
     if tape:
@@ -1054,8 +1072,8 @@ def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_
             _is_tensor(v, name)
             if v.dtype != torch.float32 or tuple(v.shape) != (M,) or not v.is_contiguous():
                 raise ValueError(f"magnet_amd: {name} must be contiguous fp32 of shape ({M},)")
-    _on_device(gy=gy, gh=gh, post=pg, post_bias=pb, pre=qg, pre_bias=qb, gate=gate, scale=sv, post_tape=post_tape,
-               post_rstd=post_rstd if pg is not None else None, pre_tape=pre_tape if qg is not None else None, pre_rstd=pre_rstd if qg is not None else None)
+    _on_device(gy, gh, pg, pb, qg, qb, gate, sv, post_tape, post_rstd if pg is not None else None, pre_tape if qg is not None else None,
+               pre_rstd if qg is not None else None)
     dev = gy.device
     fill = torch.empty if M else torch.zeros                # (no rows: no launch)
     new = lambda *s: fill(*s, dtype=gy.dtype, device=dev)  # noqa: E731
@@ -1064,7 +1082,7 @@ def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_
                       (par(pg), par(pb)) if pg is not None else None, (par(qg), par(qb)) if qg is not None else None)
     if M == 0:
         return g
-    ws = torch.empty(_floats("magnet_norm_join_bwd_workspace", C.c_long(M), W, C.c_long(G)), device=dev, dtype=torch.float32)
+    ws = torch.empty(_floats("magnet_norm_join_bwd_workspace", M, W, G), device=dev, dtype=torch.float32)
     post_g, pre_g = g.post or (None, None), g.pre or (None, None)
     L.check(L.lib().magnet_norm_join_bwd(_p(gy), _ld(gy), _p(gh), _ld(gh) if gh is not None else C.c_long(0), _T8_DTYPES[gy.dtype], C.c_long(M), W,
                                          int(norm == "layer"), _p(pg), _p(pb), _p(qg), _p(qb), _p(gate), _ld(gate) if gate is not None else C.c_long(0),

@@ -129,7 +129,7 @@ def test_c_entries_refuse():
     assert L.magnet_tape8_pack(one, 0, long(4), long(1), 4, 0, C.c_void_p(8), one, z) == -2
     assert L.magnet_tape8_pack(one, 0, long(4), long(0), 4, 0, one, one, z) == 0           # no rows: nothing to do
     assert L.magnet_tape8_unpack(one, one, long(-1), 4, 0, one, 0, long(4), z) == -2
-    assert L.magnet_tape8_linear_bwd_workspace(long(100), 0, 4, C.byref(n)) == -2
-    assert L.magnet_tape8_linear_bwd_workspace(long(100), 128, 128, C.byref(n)) == 0 and n.value == 4 * (128 * 128 + 128)
-    assert L.magnet_norm_join_bwd_workspace(long(100), 128, long(3), C.byref(n)) == -2      # 3 gates for 100 rows
-    assert L.magnet_norm_join_bwd_workspace(long(100), 4097, long(0), C.byref(n)) == -2
+    assert L.magnet_tape8_linear_bwd_workspace(long(100), long(0), long(4), C.byref(n)) == -2
+    assert L.magnet_tape8_linear_bwd_workspace(long(100), long(128), long(128), C.byref(n)) == 0 and n.value == 4 * (128 * 128 + 128)
+    assert L.magnet_norm_join_bwd_workspace(long(100), long(128), long(3), C.byref(n)) == -2      # 3 gates for 100 rows
+    assert L.magnet_norm_join_bwd_workspace(long(100), long(4097), long(0), C.byref(n)) == -2
