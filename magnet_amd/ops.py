@@ -781,6 +781,25 @@ def mpnn_readout_bwd(h, dout, tw, w1, b1, k1, s1, w2, k2, use_swish, dt):
 
 
 # ------------------------------------------------------------------------------------ 8-bit tape
+_ENTRIES: dict = {}
+_SIG = {"p": C.c_void_p, "l": C.c_long, "i": C.c_int, "f": C.c_float}
+
+
+def _entry(name, sig):
+    """an entry point with its argument types declared (p pointer, l long, i int, f float), the stream behind them: plain numbers and addresses
+    go in - a third of the host time of a small launch was ctypes objects made one by one"""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = getattr(L.lib(), name)
+        fn.argtypes = [_SIG[c] for c in sig] + [C.c_void_p]
+        _ENTRIES[name] = fn
+    return fn
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 TAPE8_KINDS = {"signed": 0, "relu": 1}
 _T8_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _T8_ACTS = {"none": ACT_NONE, "relu": ACT_RELU, "swish": ACT_SWISH}
@@ -868,8 +887,8 @@ def _matrix(t, name, dtypes, shape=None):
 
 
 def _ld(t):
-    """elements from one row to the next (of one row at least its width: torch reports any stride there)"""
-    return C.c_long(max(t.stride(0), t.shape[1]))
+    """elements from one row to the next (of one row at least its width: torch reports any stride there); 0: no tensor"""
+    return 0 if t is None else max(t.stride(0), t.shape[1])
 
 
 def _out_matrix(t, name, dtype, shape, device):
@@ -902,7 +921,8 @@ def tape8_pack(x, kind="signed", out=None) -> Tape8:
     _on_device(x, t)
     if t is None:
         t = tape8_empty(M, W, kind, x.device)
-    L.check(L.lib().magnet_tape8_pack(_p(x), _T8_DTYPES[x.dtype], _ld(x), C.c_long(M), W, TAPE8_KINDS[kind], _p(t.codes), _p(t.bytes), _stream()), "tape8_pack")
+    L.check(_entry("magnet_tape8_pack", "pilliipp")(x.data_ptr(), _T8_DTYPES[x.dtype], _ld(x), M, W, TAPE8_KINDS[kind], t.codes.data_ptr(), t.bytes.data_ptr(),
+                                                    _raw_stream(_cur_dev())), "tape8_pack")
     return t
 
 
@@ -914,8 +934,8 @@ def tape8_unpack(t: Tape8, dtype=torch.float32, out=None):
     _on_device(t)
     y = _out_matrix(out, "out", dtype, (t.rows, t.width), t.codes.device)
     _on_device(y)
-    L.check(L.lib().magnet_tape8_unpack(_p(t.codes), _p(t.bytes), C.c_long(t.rows), t.width, TAPE8_KINDS[t.kind], _p(y), _T8_DTYPES[dtype], _ld(y), _stream()),
-            "tape8_unpack")
+    L.check(_entry("magnet_tape8_unpack", "pplii" "pil")(t.codes.data_ptr(), t.bytes.data_ptr(), t.rows, t.width, TAPE8_KINDS[t.kind], y.data_ptr(),
+                                                         _T8_DTYPES[dtype], _ld(y), _raw_stream(_cur_dev())), "tape8_unpack")
     return y
 
 
@@ -961,9 +981,9 @@ def tape8_linear_bwd(dz, tape: Tape8, w, act="none", *, need_dx=True, dx=None, d
     dW = torch.empty(N, K, dtype=torch.float32, device=dev) if dW is None else dW
     db = torch.empty(N, dtype=torch.float32, device=dev) if db is None else db
     ws = torch.empty(_floats("magnet_tape8_linear_bwd_workspace", M, N, K), device=dev, dtype=torch.float32)
-    L.check(L.lib().magnet_tape8_linear_bwd_f32(_p(dz), _ld(dz), _p(tape.codes), _p(tape.bytes), _p(w), _ld(w), C.c_long(M), N, K, _T8_ACTS[act],
-                                                _p(dx), _ld(dx) if dx is not None else C.c_long(0), _p(dW), _ld(dW), _p(db), int(bool(accumulate)), _p(ws),
-                                                _stream()), "tape8_linear_bwd")
+    L.check(_entry("magnet_tape8_linear_bwd_f32", "plpppll" "iii" "plplpip")(
+        dz.data_ptr(), _ld(dz), tape.codes.data_ptr(), tape.bytes.data_ptr(), w.data_ptr(), _ld(w), M, N, K, _T8_ACTS[act], _at(dx), _ld(dx),
+        dW.data_ptr(), _ld(dW), db.data_ptr(), int(bool(accumulate)), ws.data_ptr(), _raw_stream(_cur_dev())), "tape8_linear_bwd")
     return dx, dW, db
 
 
@@ -1048,10 +1068,10 @@ def norm_join(x, f, *, post=None, pre=None, gate=None, scale=1.0, norm="layer", 
         if qg is not None:
             r.pre_tape, r.pre_rstd = tape8_empty(M, W, "signed", dev), torch.empty(M, dtype=torch.float32, device=dev)
     pt, qt = r.post_tape, r.pre_tape
-    L.check(L.lib().magnet_norm_join(_p(x), _ld(x), _p(f), _ld(f), _T8_DTYPES[x.dtype], C.c_long(M), W, int(norm == "layer"), C.c_float(float(eps)),
-                                     _p(pg), _p(pb), _p(qg), _p(qb), _p(gate), _ld(gate) if gate is not None else C.c_long(0), C.c_long(G), _p(sv),
-                                     C.c_float(sc), _p(r.y), _p(r.h), _p(pt.codes if pt else None), _p(pt.bytes if pt else None), _p(r.post_rstd),
-                                     _p(qt.codes if qt else None), _p(qt.bytes if qt else None), _p(r.pre_rstd), _stream()), "norm_join")
+    L.check(_entry("magnet_norm_join", "plpliliif" "ppppp" "llpf" "pp" "pppppp")(
+        x.data_ptr(), _ld(x), f.data_ptr(), _ld(f), _T8_DTYPES[x.dtype], M, W, int(norm == "layer"), float(eps), _at(pg), _at(pb), _at(qg), _at(qb), _at(gate),
+        _ld(gate), G, _at(sv), sc, r.y.data_ptr(), _at(r.h), _at(pt.codes if pt else None), _at(pt.bytes if pt else None), _at(r.post_rstd),
+        _at(qt.codes if qt else None), _at(qt.bytes if qt else None), _at(r.pre_rstd), _raw_stream(_cur_dev())), "norm_join")
     return r
 
 
@@ -1084,12 +1104,12 @@ def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_
         return g
     ws = torch.empty(_floats("magnet_norm_join_bwd_workspace", M, W, G), device=dev, dtype=torch.float32)
     post_g, pre_g = g.post or (None, None), g.pre or (None, None)
-    L.check(L.lib().magnet_norm_join_bwd(_p(gy), _ld(gy), _p(gh), _ld(gh) if gh is not None else C.c_long(0), _T8_DTYPES[gy.dtype], C.c_long(M), W,
-                                         int(norm == "layer"), _p(pg), _p(pb), _p(qg), _p(qb), _p(gate), _ld(gate) if gate is not None else C.c_long(0),
-                                         C.c_long(G), _p(sv), C.c_float(sc), _p(post_tape.codes), _p(post_tape.bytes),
-                                         _p(post_rstd if pg is not None else None), _p(pre_tape.codes if qg is not None else None),
-                                         _p(pre_tape.bytes if qg is not None else None), _p(pre_rstd if qg is not None else None), _p(g.x), _p(g.f),
-                                         _p(g.gate), _p(g.scale), _p(post_g[0]), _p(post_g[1]), _p(pre_g[0]), _p(pre_g[1]), _p(ws), _stream()),
+    has_post, has_pre = pg is not None, qg is not None
+    L.check(_entry("magnet_norm_join_bwd", "plplilii" "ppppp" "llpf" "pppppp" "ppp" "ppppp" "p")(
+        gy.data_ptr(), _ld(gy), _at(gh), _ld(gh), _T8_DTYPES[gy.dtype], M, W, int(norm == "layer"), _at(pg), _at(pb), _at(qg), _at(qb), _at(gate), _ld(gate), G,
+        _at(sv), sc, post_tape.codes.data_ptr(), post_tape.bytes.data_ptr(), _at(post_rstd if has_post else None), _at(pre_tape.codes if has_pre else None),
+        _at(pre_tape.bytes if has_pre else None), _at(pre_rstd if has_pre else None), g.x.data_ptr(), g.f.data_ptr(), _at(g.gate), _at(g.scale), _at(post_g[0]),
+        _at(post_g[1]), _at(pre_g[0]), _at(pre_g[1]), ws.data_ptr(), _raw_stream(_cur_dev())),
             "norm_join_bwd")
     return g
 
