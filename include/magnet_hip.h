@@ -571,7 +571,9 @@ int magnet_norm_join(const void* x, long ldx, const void* f, long ldf, int dtype
                      const float* post_b, const float* pre_g, const float* pre_b, const void* gate, long ldg, long G, const float* scale_v,
                      float scale, void* y, void* h, void* post_codes, void* post_bytes, float* post_rstd, void* pre_codes, void* pre_bytes,
                      float* pre_rstd, void* stream);
-/* Its backward from gy = d y, gh = d h (pre norm only) and the tapes: dx, df [M][W], dgate [G][W] (dtype), d_scale / d_post_g / d_post_b /
+/* The tape of a norm that ran elsewhere: the rows of z before gain and bias onto a signed tape, 1 / sqrt(..) into rstd [M]. */
+int magnet_norm_tape(const void* z, long ldz, int dtype, long M, int W, int layer, float eps, void* codes, void* bytes, float* rstd, void* stream);
+/* Its backward (of magnet_norm_join) from gy = d y, gh = d h (pre norm only) and the tapes: dx (NULL: not wanted), df [M][W], dgate [G][W] (dtype), d_scale / d_post_g / d_post_b /
  * d_pre_g / d_pre_b [W] (fp32, written; NULL: not wanted).  M >= 1.  workspace: magnet_norm_join_bwd_workspace(M, W, G or 0) floats.  The sums
  * over rows are added in a fixed order. */
 int magnet_norm_join_bwd_workspace(long M, long W, long G, long* floats);

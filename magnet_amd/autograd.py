@@ -5,6 +5,8 @@ kernel, so each one is wrapped in a ``torch.autograd.Function`` whose backward i
 only chains them and differentiates the data movement in between (``cat`` / ``permute`` / ``reshape`` / slicing), which
 keeps the rollout feedback (``models/magnet_gnn.py:442-475``) differentiable without bespoke glue.
 
+``norm_join``: a residual block's end and the next one's norm in one pass.  ``with tape8():`` keeps the chains' tapes in 8 bits.
+
 ``mlp`` is the workhorse: the fused gather/concat -> N x (Linear + ReLU) -> [LayerNorm] -> store | +residual | CSR-mean
 kernel.  Its forward is the inference kernel; when the backward's tape (assembled first-layer input, hidden activations,
 pre-LayerNorm output) fits in memory the same launch writes it (``_keep_tape``), else the backward recomputes the chain with one
@@ -75,6 +77,28 @@ class accumulate_param_grads:
 
     def __exit__(self, *exc):
         _ACCUM["on"] = self.prev
+        return False
+
+
+_TAPE8 = {"on": False}
+
+
+class tape8:
+    """``with tape8():`` around the forward of a training step: the MLP chains built inside keep their tape in 8 bits (ops.Tape8) - every
+    hidden activation as codes that carry the ReLU mask exactly, the normalised row in place of the LayerNorm's input - and their
+    backward walks the hidden Linears back from it (ops.tape8_linear_bwd).  A quarter of the memory between forward and backward, and gradients of
+    the same function with activations rounded to a step of at most 2 / 255 of their block's largest value.  ``tape8(False)``: off inside."""
+
+    def __init__(self, on=True):
+        self.on = bool(on)
+
+    def __enter__(self):
+        self.prev = _TAPE8["on"]
+        _TAPE8["on"] = self.on
+        return self
+
+    def __exit__(self, *exc):
+        _TAPE8["on"] = self.prev
         return False
 
 
@@ -392,7 +416,7 @@ class _Mlp(torch.autograd.Function):
             m.x0_dense = _x0_not_needed(m, srcs, m.M, np0, fk)        # the decision travels with the tape (not re-derived from the
             x0_free = m.x0_dense is not None                          # environment in the backward)
             K0t = 0 if x0_free else K0
-        if wants_tape and _keep_tape(4 * m.M * (K0t + (nl - 1) * pk.ht * 32 + pk.ot * 32), y.device):
+        if wants_tape and _keep_tape(m.M * (4 * K0t + ((nl - 1) * pk.ht * 32 + pk.ot * 32) * (33 / 32 if m.tape8 else 4)), y.device):
             new = lambda w: torch.empty(m.M, w, device=y.device, dtype=torch.float32)  # noqa: E731
             tape = (new(K0t), *[new(pk.ht * 32) for _ in range(nl - 1)], *([new(pk.ot * 32)] if pk.ln is not None else []))
             seg = dict(seg, x0_out=None if x0_free else tape[0], hid=list(tape[1:nl]) + [tape[nl] if pk.ln is not None else None],
@@ -401,6 +425,18 @@ class _Mlp(torch.autograd.Function):
                 last_act=m.final_relu, ln=pk.ln, epi=m.epi, y=y, res=res, ncols=pk.out_dim, **seg)
         if m.epi == ops.EPI_SEGMEAN:
             ops.segmean_fixup(m.rowptr, m.out_rows, pk.ot * 32, seg["partials"], y)
+        ctx.tape8 = bool(tape) and m.tape8
+        if ctx.tape8:                                                    # the activations onto the 8-bit tape; what the launch wrote is let go
+            params = tensors[m.n_src:m.n_src + m.n_par]
+            seg = None
+            t8 = [tape[0]]
+            for l in range(1, nl):
+                t = ops.tape8_pack(tape[l][:, :params[2 * l].shape[1]], "relu")
+                t8 += [t.codes, t.bytes]
+            if pk.ln is not None:
+                t, rstd = ops.norm_tape(tape[nl][:, :pk.out_dim], "layer", pk.ln[2])
+                t8 += [t.codes, t.bytes, rstd]
+            tape = tuple(t8)
         ctx.meta = m
         ctx.n_tape = len(tape)
         ctx.save_for_backward(*tensors, *([y] if m.final_relu else []), *tape)
@@ -428,7 +464,7 @@ class _Mlp(torch.autograd.Function):
         with torch.no_grad():
             # ---- epilogue
             d_res = dy if m.has_res else None
-            mean_in_ln = m.epi == ops.EPI_SEGMEAN and pk.ln is not None and dy.shape[1] == Dp      # the LayerNorm backward gathers dy[tgt] / deg itself
+            mean_in_ln = m.epi == ops.EPI_SEGMEAN and pk.ln is not None and dy.shape[1] == Dp and not ctx.tape8    # the LayerNorm backward gathers dy[tgt] / deg itself
             if mean_in_ln:
                 d_rows = None
             elif m.epi == ops.EPI_SEGMEAN:
@@ -448,8 +484,8 @@ class _Mlp(torch.autograd.Function):
             zL = None
             x0_dense = None                                               # {k tile: (source, column, scale)} when x0 does not exist
             if tape:                                                      # kept by the forward launch
-                x0, X = tape[0], list(tape[:nl])
-                zL = tape[nl] if pk.ln is not None else None
+                x0, X = tape[0], list(tape[:1 if ctx.tape8 else nl])
+                zL = tape[nl] if pk.ln is not None and not ctx.tape8 else None
                 if x0.numel() == 0 and M > 0:
                     x0_dense = m.x0_dense                                 # what the forward decided when it left x0 out of the tape
                     assert x0_dense is not None
@@ -468,7 +504,12 @@ class _Mlp(torch.autograd.Function):
                 X = [x0]
                 if pk.ln is not None:
                     zL = _linear(M, X[-1], pk.layers[nl - 1], pk.ot, relu=False)
-            if pk.ln is not None:
+            if ctx.tape8:
+                ln_amax = None
+                dz, d_ln = _walk_back_tape8(ctx, m, pk, params, tape, d_rows)
+                if d_ln is not None:
+                    grads_par[2 * nl], grads_par[2 * nl + 1] = d_ln
+            elif pk.ln is not None:
                 nblk = min(2048, (M + 3) // 4)
                 part = torch.empty(nblk, 2, D, device=dev, dtype=torch.float32)
                 # (the kernel writes the D real columns of every row; padding columns, if any, must read as zero)
@@ -497,17 +538,18 @@ class _Mlp(torch.autograd.Function):
                 return (l_ > 0 and tuple(W_.shape) == (Np_, Np_) and X[l_].shape[1] == Np_ and Np_ in (128, 64) and M >= _FUSED_LAYER_ROWS
                         and pk.layers[0][0].dtype == torch.float16 and X[l_].is_contiguous())
 
-            def grad_dest(W_, b_, Np_):
+            def grad_dest(W_, b_, Np_, Kp_=None):
                 """(dW, db, accumulate, into): the parameter's own .grad when accumulate_param_grads lets the kernel's reduction add to it"""
                 # (a frozen Linear - requires_grad=False tensors are leaves too - must not get a .grad from here: autograd drops
                 #  what backward returns for it, an optimizer built over self.parameters() would not drop an assigned .grad)
+                Kp_ = Np_ if Kp_ is None else Kp_
                 into_ = (m.accum and takes_inplace_grad(W_) and takes_inplace_grad(b_)
-                         and W_.dtype == b_.dtype == torch.float32 and tuple(W_.shape) == (Np_, Np_) and tuple(b_.shape) == (Np_,))
+                         and W_.dtype == b_.dtype == torch.float32 and tuple(W_.shape) == (Np_, Kp_) and tuple(b_.shape) == (Np_,))
                 Wg_, bg_ = (W_.grad, b_.grad) if into_ else (None, None)
                 if (Wg_ is not None and bg_ is not None and Wg_.dtype == bg_.dtype == torch.float32 and Wg_.device == bg_.device == dev
                         and Wg_.is_contiguous() and bg_.is_contiguous()):
                     return Wg_, bg_, True, into_
-                return (torch.empty(Np_, Np_, device=dev, dtype=torch.float32), torch.empty(Np_, device=dev, dtype=torch.float32), False, into_)
+                return (torch.empty(Np_, Kp_, device=dev, dtype=torch.float32), torch.empty(Np_, device=dev, dtype=torch.float32), False, into_)
 
             def grad_place(l_, W_, b_, dWp_, dbp_, accumulated, into_):
                 if accumulated:
@@ -517,8 +559,16 @@ class _Mlp(torch.autograd.Function):
                 else:
                     grads_par[2 * l_], grads_par[2 * l_ + 1] = dWp_, dbp_
 
+            if ctx.tape8:
+                for l in range(nl - 1, 0, -1):
+                    W, b = params[2 * l], params[2 * l + 1]
+                    dWl, dbl, acc, into = grad_dest(W, b, *W.shape)
+                    t = ops.Tape8(tape[2 * l - 1], tape[2 * l], W.shape[1], "relu")
+                    dz = ops.tape8_linear_bwd(dz, t, W.detach().float(), "relu", dW=dWl, db=dbl, accumulate=acc)[0]
+                    grad_place(l, W, b, dWl, dbl, acc, into)
+                dz = _pad_cols(dz, pk.ht * 32)
             skip = False
-            for l in range(nl - 1, -1, -1):
+            for l in range(0 if ctx.tape8 else nl - 1, -1, -1):
                 if skip:                                                  # (walked back together with the layer above it)
                     skip = False
                     continue
@@ -744,6 +794,19 @@ class _Mlp(torch.autograd.Function):
         return (None, *grads_src, *grads_par, *([d_res] if m.has_res else []))
 
 
+def _walk_back_tape8(ctx, m, pk, params, tape, d_rows):
+    """the gradient at the last Linear's output from the one behind the LayerNorm (if there is one) and the 8-bit tape of its normalised
+    rows -> ([M, out_dim], (d gain, d bias) or None)"""
+    D, nl = pk.out_dim, len(pk.layers)
+    d = d_rows[:, :D]
+    if pk.ln is None:
+        return d, None
+    codes, byte, rstd = tape[2 * nl - 1:2 * nl + 2]
+    gain, bias = (params[2 * nl + i].detach().float() for i in (0, 1))
+    g = ops.norm_join_bwd(d, post_tape=ops.Tape8(codes, byte, D, "signed"), post_rstd=rstd, post=(gain, bias), norm="layer", need_x=False)
+    return g.f, g.post
+
+
 def _dense_source_of_block(m, srcs, ctx, M, c0, w, factored):
     """(source, scale) when the column block [c0, c0 + w) of the first Linear's input gradient IS that source's gradient - it enters the
     chain as one dense full-width run at exactly these columns, scaled by a power of two at most (folded into the transposed pack) -
@@ -941,11 +1004,54 @@ def mlp(M, groups, pk, params, *, epi=ops.EPI_STORE, res=None, csr=None, out_row
         M=int(M), tiles=tiles, runs=runs, pk=pk, epi=epi, n_src=len(srcs), n_par=len(params), has_res=res is not None,
         tgt=csr.tgt if csr is not None else None, rowptr=csr.rowptr if csr is not None else None,
         out_rows=int(out_rows if out_rows is not None else M), first_cols=first_cols, col_map=getattr(pk, "col_map", None),
-        inv_cache={}, final_relu=bool(final_relu), grad_chain=grad_chain, accum=_ACCUM["on"])
+        inv_cache={}, final_relu=bool(final_relu), grad_chain=grad_chain, accum=_ACCUM["on"], tape8=_TAPE8["on"])
     assert not (final_relu and (pk.ln is not None or epi != ops.EPI_STORE))
     srcs = [ops._f32(s, "mlp source") for s in srcs]
     extra = [ops._f32(res, "residual")] if res is not None else []
     return _Mlp.apply(meta, *srcs, *params, *extra)
+
+
+# ------------------------------------------------------------------------------------------------ norms around a residual block
+class _NormJoin(torch.autograd.Function):
+    """ops.norm_join; its tape - the normalised rows in 8 bits - is all that stays for the backward"""
+
+    @staticmethod
+    def forward(ctx, meta, x, f, gate, scale, post_g, post_b, pre_g, pre_b):
+        post = (post_g, post_b) if post_g is not None else None
+        pre = (pre_g, pre_b) if pre_g is not None else None
+        r = ops.norm_join(x, f, post=post, pre=pre, gate=gate, scale=meta.scale if scale is None else scale, norm=meta.norm, eps=meta.eps,
+                          tape=any(ctx.needs_input_grad[1:]))
+        ctx.meta = meta
+        if r.post_tape is not None:
+            pt, qt = r.post_tape, r.pre_tape
+            ctx.save_for_backward(gate, scale, post_g, post_b, pre_g, pre_b, pt.codes, pt.bytes, r.post_rstd, qt.codes if qt else None, qt.bytes if qt else None,
+                                  r.pre_rstd)
+            ctx.width = pt.width
+        return r.y, r.h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy, gh):
+        gate, scale, post_g, post_b, pre_g, pre_b, pc, pb, pr, qc, qb, qr = ctx.saved_tensors
+        m, W = ctx.meta, ctx.width
+        g = ops.norm_join_bwd(gy, gh if pre_g is not None else None, post_tape=ops.Tape8(pc, pb, W, "signed"), post_rstd=pr,
+                              pre_tape=ops.Tape8(qc, qb, W, "signed") if qc is not None else None, pre_rstd=qr,
+                              post=(post_g, post_b) if post_g is not None else None, pre=(pre_g, pre_b) if pre_g is not None else None,
+                              gate=gate, scale=m.scale if scale is None else scale, norm=m.norm)
+        return (None, g.x, g.f, g.gate, g.scale, *(g.post or (None, None)), *(g.pre or (None, None)))
+
+
+def norm_join(x, f, *, post=None, pre=None, gate=None, scale=1.0, norm="layer", eps=1e-5):
+    """differentiable ``ops.norm_join`` -> (y, h): y = x + scale * gate * post(f), h = pre(y) (None without ``pre``).  Gradients of x, f, gate,
+    scale (a tensor) and the norms' gains and biases; between forward and backward only the normalised rows stay, in 8 bits."""
+    post_g, post_b = post if post is not None else (None, None)
+    pre_g, pre_b = pre if pre is not None else (None, None)
+    if gate is not None and isinstance(gate, torch.Tensor) and gate.dim() == 1:
+        gate = gate.unsqueeze(0)
+    vec = scale if isinstance(scale, torch.Tensor) else None
+    meta = types.SimpleNamespace(scale=None if vec is not None else float(scale), norm=norm, eps=float(eps))
+    y, h = _NormJoin.apply(meta, x, f, gate, vec, post_g, post_b, pre_g, pre_b)
+    return y, h
 
 
 # ------------------------------------------------------------------------------------------------ small ops

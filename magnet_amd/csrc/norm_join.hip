@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join(const NjArgs 
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
             nf[i] = nj_load(f + r * a.ldf + c, a.vec, W - c);
-            nx[i] = nj_load(x + r * a.ldx + c, a.vec, W - c);
+            if (x) nx[i] = nj_load(x + r * a.ldx + c, a.vec, W - c);
             if (a.has_gate) ng[i] = nj_load(gate + gr * a.ldg + c, a.vec, W - c);
         }
     };
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join(const NjArgs 
         t8_f4 v[VPT], s[VPT], m[VPT];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            v[i] = nj_f32<T>(nf[i]), s[i] = nj_f32<T>(nx[i]);
+            v[i] = nj_f32<T>(nf[i]), s[i] = x ? nj_f32<T>(nx[i]) : t8_f4{0.f, 0.f, 0.f, 0.f};
             m[i] = a.has_gate ? sc[i] * nj_f32<T>(ng[i]) : sc[i];
         }
         g += dg, in_g += din;
@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join(const NjArgs 
             if (a.tape && lane == 0) a.post_r[row] = rs;
         }
         if (a.tape) nj_tape<TL, VPT>(v, lane, blocks, row, a.post_c, a.post_e);
+        if (!y) continue;                                                     // (the tape is all that is wanted: magnet_norm_tape)
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            t8_store4(dx + r * a.ldy + c, a.vec, W - c, D[i]);
+            if (dx) t8_store4(dx + r * a.ldy + c, a.vec, W - c, D[i]);
             T0[i] += D[i], T1[i] += D[i] * v[i];
             D[i] *= gt[i] * sc[i] * pg[i];
         }
@@ -508,12 +509,27 @@ extern "C" int magnet_norm_join(const void* x, long ldx, const void* f, long ldf
     return (int)hipGetLastError();
 }
 
+extern "C" int magnet_norm_tape(const void* z, long ldz, int dtype, long M, int W, int layer, float eps, void* codes, void* bytes, float* rstd, void* stream) {
+    if (M < 0 || W < 1 || W > NJ_MAX_W || ldz < W || (dtype != T8_F32 && dtype != T8_BF16)) return -2;
+    if (M == 0) return 0;
+    if (!codes || !bytes || !rstd) return -2;
+    NjArgs a = {};
+    a.f = z, a.post_c = (unsigned char*)codes, a.post_e = (unsigned char*)bytes, a.post_r = rstd, a.M = M, a.ldf = ldz, a.rows_per_gate = M, a.W = W;
+    a.layer = layer, a.has_post = 1, a.tape = 1, a.eps = eps;
+    const void* p[] = {z};
+    const long ld[] = {ldz};
+    a.vec = nj_vec(W, dtype == T8_F32 ? 4 : 2, p, ld, 1);
+    if (dtype == T8_F32) nj_forward<float>(a, (hipStream_t)stream);
+    else nj_forward<__bf16>(a, (hipStream_t)stream);
+    return (int)hipGetLastError();
+}
+
 extern "C" int magnet_norm_join_bwd(const void* gy, long ldgy, const void* gh, long ldgh, int dtype, long M, int W, int layer, const float* post_g,
                                     const float* post_b, const float* pre_g, const float* pre_b, const void* gate, long ldg, long G, const float* scale_v,
                                     float scale, const void* post_codes, const void* post_bytes, const float* post_rstd, const void* pre_codes,
                                     const void* pre_bytes, const float* pre_rstd, void* dx, void* df, void* dgate, float* d_scale, float* d_post_g,
                                     float* d_post_b, float* d_pre_g, float* d_pre_b, float* workspace, void* stream) {
-    if (M < 1 || W < 1 || W > NJ_MAX_W || ldgy < W || (dtype != T8_F32 && dtype != T8_BF16) || !dx || !df || (gate && (G < 1 || M % G || ldg < W || !dgate)))
+    if (M < 1 || W < 1 || W > NJ_MAX_W || ldgy < W || (dtype != T8_F32 && dtype != T8_BF16) || !df || (gate && (G < 1 || M % G || ldg < W || !dgate)))
         return -2;
     if (!post_codes || !post_bytes || (post_g && !post_rstd) || (pre_g && (!gh || ldgh < W || !pre_codes || !pre_bytes || !pre_rstd))) return -2;
     const size_t size = dtype == T8_F32 ? 4 : 2;

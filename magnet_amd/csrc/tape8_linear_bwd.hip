@@ -62,7 +62,8 @@ __device__ __forceinline__ float t8_swish(float v, float& d) {
 }
 
 #define T8_WAVES(NP, KP) ((NP) == 128 && (KP) == 128 ? 8 : 4)
-#define T8_ROWS(NP, KP, ACT) ((ACT) != ACT_SWISH ? 64 : 32)      // rows of a step
+#define T8_ROWS(NP, KP, ACT) ((NP) == (KP) && (ACT) != ACT_SWISH ? 64 : 32)      // rows of a step
+#define T8_TILE(NP, KP, ACT) ((NP) == 128 && (KP) == 128 && (ACT) == ACT_SWISH ? 1 : 2)       // blocks of 16 features of a wave's tiles
 #define T8_ZROOM 3                       // binades of dz and of the tape's bytes that may still come before the scale has to change
 #define T8_XROOM 2
 template <int NP, int KP, int XPL, int R, int ACT>
@@ -87,8 +88,9 @@ __device__ __forceinline__ void t8_put(void* base, unsigned off, const V& v) {
 
 // FULL: N = NP, K a multiple of KP, dz and dx in 16-byte accesses, one block of N - no lane ever looks at a column that is not there, and
 // addresses are a uniform base and one offset (the registers that bounds and addresses take are what decides between spilling and not)
-// A workgroup of NP and KP at most 64 has four waves, else eight: a wave owns one block of 16 features of either side (of 64 features on
-// one side, every other wave the rows' other half).
+// 128 x 128 has eight waves, the smaller shapes four.  A wave's tiles are near square - 32 features of x by half the rows for dx, 32 features
+// of dz by 64 of x for dW - because what a tile needs from LDS is its two edges: 524 us at 2 097 152 rows, 537 with sixteen features by all
+// rows for each wave.  Behind Swish, where a step has half the rows, it is the other way round: 105 us against 118 at 262 144 rows.
 template <int NP, int KP, int ACT, bool FULL>
 __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(const T8LinArgs a) {
     constexpr int KIND = ACT == ACT_RELU ? T8_RELU : T8_SIGNED;
@@ -98,13 +100,19 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     constexpr int NW = T8_WAVES(NP, KP), LANES = 64 * NW;
     constexpr int LPR = NP / 4, RPL = LANES / LPR, NLD = R / RPL;             // lanes per row of dz, rows per pass, passes
     constexpr int CPT = R * KP / LANES, CPR = KP / CPT, CW = CPT / 4;        // codes per lane (8 or 16), lanes per row, words
-    constexpr int NBK = KP / 16 / NW, NBN = NP / 16 / NW, NT = NP / 32, KB = KP / 16;   // a wave's blocks of 16 features of x / of dz
+    // a wave's part: dx of NBK blocks of 16 features and 1 / RW of the rows; dW of NBN blocks of features of dz and KB of features of x
+    constexpr int NBK = T8_TILE(NP, KP, ACT), NBN = NBK, NT = NP / 32;
+    constexpr int KW = KP / 16 / NBK, RW = NW / KW, RBS = R / 16 / RW, RB = RBS < 2 ? RBS : 2;
+    constexpr int NG = NP / 16 / NBN, XG = NW / NG, KB = KP / 16 / XG;
+    static_assert(KW * RW == NW && NG * XG == NW && RBS * 16 * RW == R, "waves tile both products");
     typedef unsigned t8_cw __attribute__((ext_vector_type(CW)));
     __shared__ __attribute__((aligned(16))) Step sb[2];
     __shared__ unsigned red[NW], flag[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
     const int k0 = blockIdx.y * KP;
+    const int kf = 16 * NBK * (wave % KW), wr = (wave / KW) * (R / RW);       // its features and rows of dx
+    const int nf = 16 * NBN * (wave % NG), xf = 16 * KB * (wave / NG);        // its features of dz and of x in dW
     // ---- what this lane loads of a step
     const int zr = tid / LPR, zc = 4 * (tid % LPR);
     const int cr = tid / CPR, cc = CPT * (tid % CPR);
@@ -148,9 +156,9 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     int we;                                                                   // W is staged times 2^(140 - we): max |W| -> [2^13, 2^14)
     {
         auto w_at = [&](int b, int t, int j) -> float {
-            const int n = 32 * t + 8 * q4 + j, k = k0 + 16 * (NBK * wave + b) + n16;
+            const int n = 32 * t + 8 * q4 + j, k = k0 + kf + 16 * b + n16;
             if (FULL) {
-                const float* p = a.w + (32 * t + j) * a.ldw + k0 + 16 * (NBK * wave + b);
+                const float* p = a.w + (32 * t + j) * a.ldw + k0 + kf + 16 * b;
                 T8_UNIFORM(p);
                 return t8_at<float>(p, ((unsigned)(8 * q4) * (unsigned)a.ldw + n16) * 4u);
             }
@@ -281,18 +289,20 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
         asm volatile("" ::: "memory");
         load(min(step + (long)gridDim.x, nsteps - 1));                        // (past the last step: rows that nobody uses)
         asm volatile("" ::: "memory");
-        // ---- dx, 32 rows at a time: dx^T, acc[b][rb] = features 16 (NBK wave + b) .. of rows 16 rb ..
+        // ---- dx^T: acc[b][rb] = features kf + 16 b .. of rows wr + 16 (rp + rb) ..
 #pragma unroll
-        for (int r32 = 0; r32 < R; r32 += 32) {
-            f32x4 acc[NBK][2];
+        for (int rp = 0; rp < RBS; rp += RB) {
+            f32x4 acc[NBK][RB];
 #pragma unroll
-            for (int b = 0; b < NBK; ++b) acc[b][0] = acc[b][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int b = 0; b < NBK; ++b)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) acc[b][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int rb = 0; rb < 2; ++rb) {
-                    const t8_h8 zh = *reinterpret_cast<const t8_h8*>(&B.z[0][r32 + 16 * rb + n16][32 * t + 8 * q4]);
-                    const t8_h8 zl = *reinterpret_cast<const t8_h8*>(&B.z[1][r32 + 16 * rb + n16][32 * t + 8 * q4]);
+                for (int rb = 0; rb < RB; ++rb) {
+                    const t8_h8 zh = *reinterpret_cast<const t8_h8*>(&B.z[0][wr + 16 * (rp + rb) + n16][32 * t + 8 * q4]);
+                    const t8_h8 zl = *reinterpret_cast<const t8_h8*>(&B.z[1][wr + 16 * (rp + rb) + n16][32 * t + 8 * q4]);
 #pragma unroll
                     for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl[b][t], zh, acc[b][rb], 0, 0, 0);
 #pragma unroll
@@ -301,17 +311,17 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                     for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zh, acc[b][rb], 0, 0, 0);
                 }
             __builtin_amdgcn_sched_barrier(0);                                // (without these the reads of all parts move up and the registers run out)
-            // dx = act'(v) (dz W): lane = row 16 rb + n16, features 4 q4 .. + 3 of the block
+            // dx = act'(v) (dz W): lane = row n16 of the block of rows, features 4 q4 .. + 3 of the block of features
             if (a.dx) {
                 const int e = we + ze - 280;
-                float* const bx = a.dx + (row0 + r32) * a.lddx + k0;
-                const unsigned ox = ((unsigned)n16 * (unsigned)a.lddx + 16 * NBK * wave + 4 * q4) * 4u;
+                float* const bx = a.dx + (row0 + wr + 16 * rp) * a.lddx + k0 + kf;
+                const unsigned ox = ((unsigned)n16 * (unsigned)a.lddx + 4 * q4) * 4u;
 #pragma unroll
-                for (int rb = 0; rb < 2; ++rb) {
-                    const int lr = r32 + 16 * rb + n16;                       // row of the step
+                for (int rb = 0; rb < RB; ++rb) {
+                    const int lr = wr + 16 * (rp + rb) + n16;                 // row of the step
 #pragma unroll
                     for (int b = 0; b < NBK; ++b) {
-                        const int f = 16 * (NBK * wave + b) + 4 * q4, k = k0 + f;
+                        const int f = kf + 16 * b + 4 * q4, k = k0 + f;
                         t8_f4 v;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(acc[b][rb][i], e);
@@ -342,15 +352,16 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             t8_h8 ah[NBN], al[NBN];
 #pragma unroll
             for (int b = 0; b < NBN; ++b) {
-                const int f = 16 * (NBN * wave + b) + c0;
+                const int f = nf + 16 * b + c0;
                 ah[b] = t8_join(t8_tr(&B.z[0][r0][f]), t8_tr(&B.z[0][16 + r0][f]));
                 al[b] = t8_join(t8_tr(&B.z[1][r0][f]), t8_tr(&B.z[1][16 + r0][f]));
             }
 #pragma unroll
             for (int x = 0; x < KB; ++x) {
-                const t8_h8 xh = t8_join(t8_tr(&B.x[0][r0][16 * x + c0]), t8_tr(&B.x[0][16 + r0][16 * x + c0]));
+                const int f = xf + 16 * x + c0;
+                const t8_h8 xh = t8_join(t8_tr(&B.x[0][r0][f]), t8_tr(&B.x[0][16 + r0][f]));
                 if (XPL == 2) {
-                    const t8_h8 xl = t8_join(t8_tr(&B.x[XPL - 1][r0][16 * x + c0]), t8_tr(&B.x[XPL - 1][16 + r0][16 * x + c0]));
+                    const t8_h8 xl = t8_join(t8_tr(&B.x[XPL - 1][r0][f]), t8_tr(&B.x[XPL - 1][16 + r0][f]));
 #pragma unroll
                     for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b], xl, accw[b][x], 0, 0, 0);
                 }
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                 for (int x = 0; x < KB; ++x)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float* o = wout + (16 * (NBN * wave + b) + i) * KP + 16 * x;
+                        float* o = wout + (nf + 16 * b + i) * KP + xf + 16 * x;
                         T8_UNIFORM(o);
                         const float v = __builtin_amdgcn_ldexpf(accw[b][x][i], ze + xe - 272);
                         t8_put<float>(o, ol, add ? t8_at<float>(o, ol) + v : v);

@@ -139,8 +139,8 @@ class _RolloutScope:
         from ..packing import deferred_weight_checks
         self.parts = (deferred_weight_checks(), model._guard.armed())
         if torch.is_grad_enabled() and model.training:      # a training step: loss.backward() follows (autograd.accumulate_param_grads)
-            from ..autograd import accumulate_param_grads
-            self.parts += (accumulate_param_grads(),)
+            from ..autograd import accumulate_param_grads, tape8
+            self.parts += (accumulate_param_grads(), tape8(model.tape8))
 
     def __enter__(self):
         for p in self.parts:
@@ -226,6 +226,8 @@ class MagnetBase(LightningModule):
         from ..packing import default_gemm
         self._guard = ops.RangeGuard(default_gemm() == "fp16x3" and bool(getattr(hparams, "range_check", True)))
         self.optimizer_kind = getattr(hparams, "optimizer", "fused")     # "fused" (magnet_amd.optim.FusedAdam) | "torch"
+        # the training tape in 8 bits (autograd.tape8): a quarter of the memory between forward and backward, gradients to about 1 %
+        self.tape8 = bool(getattr(hparams, "tape8", os.environ.get("MAGNET_TAPE8", "0") != "0"))
         # hipGraph replay of whole inference rollouts (magnet_amd/graphs.py): True / False / "auto" = when the graph is small
         self.hip_graph = getattr(hparams, "hip_graph", "auto")
         self._rollout_graph = RolloutGraph(topology_keys=self.TOPOLOGY_KEYS)

@@ -1002,7 +1002,7 @@ class NormJoin:
 @dataclass
 class NormJoinGrads:
     """gradients of ``norm_join``: x, f, gate, scale and the (gain, bias) pairs post and pre; None for what was not there"""
-    x: torch.Tensor
+    x: torch.Tensor | None
     f: torch.Tensor
     gate: torch.Tensor | None = None
     scale: torch.Tensor | None = None
@@ -1075,10 +1075,23 @@ def norm_join(x, f, *, post=None, pre=None, gate=None, scale=1.0, norm="layer", 
     return r
 
 
+def norm_tape(z, norm="layer", eps=1e-5):
+    """the rows of a norm before gain and bias, on an 8-bit tape, and 1 / sqrt(variance + eps): what ``norm_join_bwd`` reads of a norm that ran
+    elsewhere (``norm_join`` keeps its own) -> (Tape8, fp32 [M])"""
+    z, _, _, _, _, _, _ = _join_args(z, "z", None, None, None, 1.0, norm)
+    M, W = z.shape
+    _on_device(z)
+    t, rstd = tape8_empty(M, W, "signed", z.device), torch.empty(M, dtype=torch.float32, device=z.device)
+    L.check(_entry("magnet_norm_tape", "plilii" "fppp")(z.data_ptr(), _ld(z), _T8_DTYPES[z.dtype], M, W, int(norm == "layer"), float(eps), t.codes.data_ptr(),
+                                                        t.bytes.data_ptr(), rstd.data_ptr(), _raw_stream(_cur_dev())), "norm_tape")
+    return t, rstd
+
+
 def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_rstd=None, post=None, pre=None, gate=None, scale=1.0,
-                  norm="layer") -> NormJoinGrads:
+                  norm="layer", need_x=True) -> NormJoinGrads:
     """The backward pass of ``norm_join`` from the gradients of y and h (with a pre norm) and what its ``tape`` kept; post, pre, gate, scale and
-    norm as handed to it.  Gradients of x, f and gate have gy's type, those of parameters are fp32."""
+    norm as handed to it.  Gradients of x, f and gate have gy's type, those of parameters are fp32.  ``need_x`` False: no gradient of x
+    (without a pre norm it is gy)."""
     gy, (pg, pb), (qg, qb), gate, G, sv, sc = _join_args(gy, "gy", post, pre, gate, scale, norm)
     M, W = gy.shape
     if (gh is None) != (qg is None):
@@ -1098,7 +1111,7 @@ def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_
     fill = torch.empty if M else torch.zeros                # (no rows: no launch)
     new = lambda *s: fill(*s, dtype=gy.dtype, device=dev)  # noqa: E731
     par = lambda p: fill(W, dtype=torch.float32, device=dev) if p is not None else None  # noqa: E731
-    g = NormJoinGrads(new(M, W), new(M, W), new(*gate.shape) if gate is not None else None, par(sv),
+    g = NormJoinGrads(new(M, W) if need_x else None, new(M, W), new(*gate.shape) if gate is not None else None, par(sv),
                       (par(pg), par(pb)) if pg is not None else None, (par(qg), par(qb)) if qg is not None else None)
     if M == 0:
         return g
@@ -1108,7 +1121,7 @@ def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_
     L.check(_entry("magnet_norm_join_bwd", "plplilii" "ppppp" "llpf" "pppppp" "ppp" "ppppp" "p")(
         gy.data_ptr(), _ld(gy), _at(gh), _ld(gh), _T8_DTYPES[gy.dtype], M, W, int(norm == "layer"), _at(pg), _at(pb), _at(qg), _at(qb), _at(gate), _ld(gate), G,
         _at(sv), sc, post_tape.codes.data_ptr(), post_tape.bytes.data_ptr(), _at(post_rstd if has_post else None), _at(pre_tape.codes if has_pre else None),
-        _at(pre_tape.bytes if has_pre else None), _at(pre_rstd if has_pre else None), g.x.data_ptr(), g.f.data_ptr(), _at(g.gate), _at(g.scale), _at(post_g[0]),
+        _at(pre_tape.bytes if has_pre else None), _at(pre_rstd if has_pre else None), _at(g.x), g.f.data_ptr(), _at(g.gate), _at(g.scale), _at(post_g[0]),
         _at(post_g[1]), _at(pre_g[0]), _at(pre_g[1]), ws.data_ptr(), _raw_stream(_cur_dev())),
             "norm_join_bwd")
     return g

@@ -456,3 +456,260 @@ def test_norm_join_constant_and_not_finite_rows():
         assert torch.isnan(r.y[7]).all() and torch.isnan(r.h[7]).all() and bool((r.post_tape.bytes[7] == 255).all())
         keep = torch.arange(20, device="cuda") != 7
         assert torch.equal(r.y[keep], clean.y[keep]) and torch.equal(r.pre_tape.codes[keep], clean.pre_tape.codes[keep])
+
+
+def test_norm_tape_is_the_tape_of_norm_join():
+    from magnet_amd import ops
+    for norm in ("layer", "rms"):
+        for W, dt in ((64, torch.float32), (100, torch.bfloat16), (1500, torch.float32)):
+            c = join_case(77, W, 0, norm, True, False, False, dt)
+            want = ops.norm_join(**c, tape=True)
+            t, r = ops.norm_tape(c["f"], norm)
+            assert torch.equal(t.codes, want.post_tape.codes) and torch.equal(t.bytes, want.post_tape.bytes) and torch.equal(r, want.post_rstd)
+            g, gy = (ops.norm_join_bwd(c["x"], post_tape=t, post_rstd=r, post=c["post"], norm=norm, need_x=x) for x in (False, True))
+            assert g.x is None and torch.equal(g.f, gy.f) and torch.equal(g.post[0], gy.post[0]) and torch.equal(gy.x, c["x"])
+
+
+# --------------------------------------------------------------------------------------------------------------------- gradients
+def exact_join(c, x, f):
+    M = x.shape[0]
+    y = x + c["scale"] * ref_gate(c, M) * ref_affine(ref_norm(f, c["norm"])[0] if c["post"] else f, c["post"])
+    return y, ref_affine(ref_norm(y, c["norm"])[0], c["pre"]) if c["pre"] else None
+
+
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("uses", ["both", "y", "h"])
+@pytest.mark.parametrize("G", [0, 1, 6, 300])
+def test_norm_join_gradients(norm, uses, G):
+    """autograd.norm_join against the formula's gradients (fp64 autograd) and against differences of the formula along a direction.  What
+    the tape rounds: codes of normalised rows (deviation 1, block tops about 2.5) are off by step / sqrt(12) <= 2.5 / 127 / sqrt(12) = 0.6 %
+    of the deviation; it enters a gradient through v^ mean(u v^) and the gains' sums: a share below that of the whole.  2 % bounds it."""
+    from magnet_amd import autograd as AG
+    M, W = 300, 128
+    c = join_case(M, W, G, norm, True, True, True, torch.float32, seed=G + 1)
+    leaves = {"x": c["x"], "f": c["f"], "gate": c["gate"], "scale": c["scale"], "post_g": c["post"][0], "post_b": c["post"][1], "pre_g": c["pre"][0], "pre_b": c["pre"][1]}
+    leaves = {k: v for k, v in leaves.items() if v is not None}
+    torch.manual_seed(5)
+    wy, wh = torch.randn(M, W, device="cuda"), torch.randn(M, W, device="cuda")
+
+    def case(v):
+        return dict(c, x=v["x"], f=v["f"], gate=v.get("gate"), scale=v["scale"], post=(v["post_g"], v.get("post_b")), pre=(v["pre_g"], v.get("pre_b")))
+
+    def loss(y, h, a, b):
+        return ((y * a).sum() if uses != "h" else 0.0) + ((h * b).sum() if uses != "y" else 0.0)
+    mine = {k: v.clone().requires_grad_() for k, v in leaves.items()}
+    d = case(mine)
+    y, h = AG.norm_join(d["x"], d["f"], post=d["post"], pre=d["pre"], gate=d["gate"], scale=d["scale"], norm=norm)
+    loss(y, h, wy, wh).backward()
+    exact = {k: v.double().requires_grad_() for k, v in leaves.items()}
+    d = case(exact)
+    ye, he = exact_join(d, d["x"], d["f"])
+    near(y.detach(), ye.detach(), torch.float32)
+    near(h.detach(), he.detach(), torch.float32)
+    loss(ye, he, wy.double(), wh.double()).backward()
+    for k, v in exact.items():
+        if v.grad is None or (uses == "y" and k.startswith("pre")):
+            assert mine[k].grad is None or not mine[k].grad.any()
+            continue
+        assert mine[k].grad.dtype == mine[k].dtype and mine[k].grad.shape == mine[k].shape
+        assert float((mine[k].grad - v.grad).norm()) <= 0.02 * float(v.grad.norm()), k
+    # differences: the loss along one direction of all leaves, central, 64 bits (error of the second order in 1e-5)
+    dirs = {k: torch.randn(v.shape, device="cuda", dtype=torch.float64) for k, v in leaves.items()}
+    with torch.no_grad():
+        at = [loss(*exact_join(case({k: v + s * dirs[k] for k, v in exact.items()}), exact["x"] + s * dirs["x"], exact["f"] + s * dirs["f"]),
+                   wy.double(), wh.double()) for s in (1e-5, -1e-5)]
+        slope = float(at[0] - at[1]) / 2e-5
+        got = sum(float((mine[k].grad.double() * dirs[k]).sum()) for k in leaves if mine[k].grad is not None)
+        size = sum(float((v.grad * dirs[k]).norm()) for k, v in exact.items() if v.grad is not None)
+    assert abs(got - slope) <= 0.02 * size + 1e-6 * abs(slope), (got, slope)
+
+
+def chain_case(M, hidden, D, K, seed, ln):
+    """an MLP of five Linears on dense rows, its packed namespace and the torch parameters behind it"""
+    import types
+
+    from magnet_amd.packing import pack, pad_to
+    torch.manual_seed(seed)
+    dims = [K, hidden, hidden, hidden, hidden, D]
+    lins = [torch.nn.Linear(a, b).cuda() for a, b in zip(dims, dims[1:])]
+    norm = torch.nn.LayerNorm(D).cuda() if ln else None
+    if ln:
+        torch.nn.init.normal_(norm.weight, 1.0, 0.2)
+        torch.nn.init.normal_(norm.bias, 0.0, 0.2)
+    Dp = pad_to(D)
+    pad = lambda v: torch.nn.functional.pad(v.detach(), (0, Dp - D)).contiguous()  # noqa: E731
+    pk = types.SimpleNamespace(layers=[pack(m.weight.detach(), m.bias.detach(), "fp16x3") for m in lins], ln=(pad(norm.weight), pad(norm.bias), norm.eps) if ln else None,
+                               ht=pad_to(hidden) // 32, ot=Dp // 32, out_dim=D, col_map=None)
+    params = [p for m in lins for p in (m.weight, m.bias)] + ([norm.weight, norm.bias] if ln else [])
+    return lins, norm, pk, params, torch.randn(M, K, device="cuda")
+
+
+@pytest.mark.parametrize("M,hidden,D,K,ln", [(5000, 128, 128, 128, True), (5000, 64, 32, 64, True), (777, 128, 1, 32, False), (4500, 64, 10, 64, False)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_mlp_with_the_tape_in_8_bits(M, hidden, D, K, ln, in_place, monkeypatch):
+    """the whole chain: the forward's bits are those of the fp32 tape, the saved activations a quarter; the ReLU masks are exact, so the gradients
+    are those of the fp32 tape but for the activations' rounding: step / sqrt(12) with step <= 2 top / 255 and block tops of 32 rectified
+    normals about 2.3 sigma against 0.7 sigma of root mean square - 0.8 % - in every dW, 1 % with the LayerNorm's tape; 2.5 % bounds it"""
+    from magnet_amd import autograd as AG, ops
+    monkeypatch.setenv("MAGNET_KEEP_TAPE", "1")
+    lins, norm, pk, params, x = chain_case(M, hidden, D, K, 3, ln)
+    if ln and not ops.L.query("magnet_mlp_supported", 5, pk.ht, pk.ot, ops.ACT_RELU, 0, 1, ops.EPI_STORE):
+        pytest.skip("no such chain")
+    gy = torch.randn(M, D, device="cuda")
+    runs, kept = {}, {}
+    for on in (False, True):
+        for p in params:
+            p.grad = None
+        xi = x.clone().requires_grad_()
+        saved = []
+        if in_place:
+            with AG.tape8(on), AG.accumulate_param_grads():
+                y = AG.mlp(M, [ops.Term(xi, K)], pk, params)
+        else:
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: (saved.append(t.numel() * t.element_size()), t)[1], lambda t: t), AG.tape8(on):
+                y = AG.mlp(M, [ops.Term(xi, K)], pk, params)
+        y.backward(gy)
+        kept[on] = sum(saved) - 2 * M * K * 4 - sum(p.numel() * 4 for p in params)           # (x twice: the source and the assembled input)
+        runs[on] = [y.detach(), xi.grad] + [p.grad.clone() for p in params]
+        if in_place:                                       # a second backward of the same step adds to what is there
+            with AG.tape8(on), AG.accumulate_param_grads():
+                y2 = AG.mlp(M, [ops.Term(x.clone().requires_grad_(), K)], pk, params)
+            y2.backward(gy)
+            for p, g in zip(params, runs[on][2:]):
+                assert float((p.grad - 2 * g).norm()) <= 1e-5 * float(g.norm())
+    assert torch.equal(runs[False][0], runs[True][0])
+    assert in_place or kept[True] <= 0.27 * kept[False] + 4 * M, kept
+    for i, (a, b) in enumerate(zip(runs[True][1:], runs[False][1:])):
+        assert float((a - b).norm()) <= 0.025 * float(b.norm()), (i, float((a - b).norm() / b.norm()))
+    # and against fp64 autograd through the same chain
+    net = [m.__class__(m.in_features, m.out_features).cuda().double() for m in lins]
+    for a, b in zip(net, lins):
+        a.load_state_dict(b.state_dict())
+    x64 = x.double().requires_grad_()
+    v = x64
+    for i, m in enumerate(net):
+        v = m(v)
+        v = torch.relu(v) if i < 4 else v
+    if ln:
+        v = torch.nn.functional.layer_norm(v, (D,), norm.weight.detach().double(), norm.bias.detach().double(), norm.eps)
+    v.backward(gy.double())
+    for a, b in zip(runs[True][2:], [p.grad for m in net for p in (m.weight, m.bias)]):
+        assert float((a - b).norm()) <= 0.03 * float(b.norm())
+
+
+@pytest.mark.parametrize("teacher_forcing", [False, True])
+def test_magnet_gnn_trains_with_the_tape_in_8_bits(teacher_forcing):
+    """a model's own training step with ``tape8`` in its hparams: the loss has the bits of the fp32 tape's, every parameter a gradient within the
+    rounding of the activations (a rollout of several forwards: errors of 1 % a chain, independent from chain to chain)"""
+    from magnet_amd.models.factory import FACTORY
+    from oracle import models as O
+    from oracle.weightgen import fill_state_dict
+    from tests.helpers import load_case
+    name, hp, salt, batch, d = load_case("magnet_gnn_tiny")
+    hp.teacher_forcing = teacher_forcing
+    oracle = O.build(name, hp)
+    fill_state_dict(oracle, salt)
+    cb = {k: v.cuda() for k, v in batch.items()}
+    got = []
+    for on in (False, True):
+        hp.tape8 = on
+        model = FACTORY[name](hp)
+        model.load_state_dict(oracle.state_dict())
+        model = model.cuda().train()
+        assert model.tape8 is on
+        loss = model.training_step(cb, 0)
+        loss.backward()
+        got.append((loss.detach(), {n: p.grad for n, p in model.named_parameters()}))
+    assert torch.equal(got[0][0], got[1][0])
+    for n, g in got[0][1].items():
+        if g is None:
+            assert got[1][1][n] is None
+            continue
+        off = float((got[1][1][n] - g).norm() / g.norm()) if float(g.norm()) else 0.0
+        assert off <= 0.05, (n, off)
+
+
+# ------------------------------------------------------------------------------------------------------- together, streams, graphs
+def block(x, w1, w2, post, pre, gate, scale, gy, gh):
+    """one residual block, forward and backward, through the operators: y = x + scale gate post(relu(h0 w1^T) w2^T), h = pre(y)"""
+    from magnet_amd import ops
+    a = x @ w1.t()
+    t1 = ops.tape8_pack(a, "relu")
+    f = a.clamp(min=0) @ w2.t()
+    r = ops.norm_join(x, f, post=post, pre=pre, gate=gate, scale=scale, tape=True)
+    g = ops.norm_join_bwd(gy, gh, post_tape=r.post_tape, post_rstd=r.post_rstd, pre_tape=r.pre_tape, pre_rstd=r.pre_rstd, post=post, pre=pre, gate=gate, scale=scale)
+    da, dw2, db2 = ops.tape8_linear_bwd(g.f, t1, w2, "relu")
+    t0 = ops.tape8_pack(x)
+    dx, dw1, db1 = ops.tape8_linear_bwd(da, t0, w1)
+    return [r.y, r.h, g.x, g.f, g.gate, g.scale, *g.post, *g.pre, da, dw2, db2, dx, dw1, db1, ops.tape8_unpack(r.pre_tape)]
+
+
+def block_case(M=1500, W=128, H=96, G=3):
+    torch.manual_seed(11)
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    return dict(x=r(M, W), w1=r(H, W) / W ** 0.5, w2=r(W, H) / H ** 0.5, post=(1 + 0.1 * r(W), 0.1 * r(W)), pre=(1 + 0.1 * r(W), 0.1 * r(W)), gate=torch.sigmoid(r(G, W)),
+                scale=0.5 + 0.1 * r(W), gy=r(M, W) * 1e-6, gh=r(M, W) * 1e-6)
+
+
+def test_block_together_and_on_another_stream():
+    c = block_case()
+    want = block(**c)
+    # the block's gradients against fp64 (1 % of rounding a tape, two tapes behind one another)
+    p = {k: v.double() if isinstance(v, torch.Tensor) else tuple(u.double() for u in v) for k, v in c.items()}
+    leaves = [p["x"].requires_grad_(), p["w1"].requires_grad_(), p["w2"].requires_grad_()]
+    f = torch.relu(p["x"] @ p["w1"].t()) @ p["w2"].t()
+    ln = lambda v, q: torch.nn.functional.layer_norm(v, (v.shape[1],), q[0], q[1], EPS)  # noqa: E731
+    y = p["x"] + p["scale"] * p["gate"].repeat_interleave(500, 0) * ln(f, p["post"])
+    ((y * p["gy"]).sum() + (ln(y, p["pre"]) * p["gh"]).sum()).backward()
+    for got, ref in ((want[2] + want[13], leaves[0].grad), (want[14], leaves[1].grad), (want[11], leaves[2].grad)):
+        assert float((got - ref).norm()) <= 0.03 * float(ref.norm())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = block(**c)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_block_captured_and_replayed():
+    """two graphs of the same calls, replayed in turn with eager work between, on inputs that change: every replay has the eager bits"""
+    c, d = block_case(), block_case(M=333, W=64, H=128, G=333)
+    graphs = []
+    for e in (c, d):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block(**e)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = block(**e)
+        graphs.append((g, out, e))
+    for k in range(4):
+        for g, out, e in graphs:
+            for name in ("x", "gy", "gh"):
+                e[name].copy_(torch.randn_like(e[name]) * (1.0 if name == "x" else 10.0 ** (-6 + k)))
+            g.replay()
+            want = block(**e)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_a_backward_is_the_same_while_another_runs():
+    """two streams at work at the same time on workspaces of their own"""
+    from magnet_amd import ops
+    dz, t, w = linear_case(60000, 128, 128, "relu", seed=9)
+    want = ops.tape8_linear_bwd(dz, t, w, "relu")
+    c = join_case(40000, 128, 4, "layer", True, True, True, torch.float32)
+    r = ops.norm_join(**c, tape=True)
+    args = dict(post_tape=r.post_tape, post_rstd=r.post_rstd, pre_tape=r.pre_tape, pre_rstd=r.pre_rstd, **{k: c[k] for k in ("post", "pre", "gate", "scale", "norm")})
+    other = ops.norm_join_bwd(c["x"], c["f"], **args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            g = ops.norm_join_bwd(c["x"], c["f"], **args)
+        got = ops.tape8_linear_bwd(dz, t, w, "relu")
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(g.f, other.f) and torch.equal(g.gate, other.gate) and torch.equal(g.scale, other.scale)
