@@ -34,7 +34,7 @@ struct NjArgs {
     long M, ldx, ldf, ldg, ldy, ldh;
     long rows_per_gate;                  // M / G (M without a gate)
     long groups;                         // backward: G, 1 without a gate
-    int W, vec, layer, has_post, has_pre, has_gate, tape, per_group, need_sums;
+    int W, layer, has_post, has_pre, has_gate, tape, per_group, need_sums;
     float scale, eps;
 };
 
@@ -143,13 +143,7 @@ __device__ __forceinline__ void nj_tape(const t8_f4 (&v)[VPT], int lane, int blo
     }
 }
 // a row of parameters: fp32, zero past the width; `none` where there is none
-__device__ __forceinline__ t8_f4 nj_par(const float* p, int c, int W, float none) {
-    t8_f4 v = {none, none, none, none};
-    if (!p) return v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c + i < W ? p[c + i] : 0.f;
-    return v;
-}
+__device__ __forceinline__ t8_f4 nj_par(const float* p, int c, int W, float none) { return p ? t8_load4(p + c, W - c) : t8_f4{none, none, none, none}; }
 __device__ __forceinline__ t8_f4 nj_scale(const NjArgs& a, int c) {
     return a.scale_v ? nj_par(a.scale_v, c, a.W, 0.f) : t8_f4{a.scale, a.scale, a.scale, a.scale};
 }
@@ -157,11 +151,11 @@ __device__ __forceinline__ t8_f4 nj_scale(const NjArgs& a, int c) {
 template <typename T>
 using nj_raw = T __attribute__((ext_vector_type(4)));
 template <typename T>
-__device__ __forceinline__ nj_raw<T> nj_load(const T* __restrict__ p, bool vec, int n) {
-    if (vec) return n > 0 ? *reinterpret_cast<const nj_raw<T>*>(p) : nj_raw<T>(0);
+__device__ __forceinline__ nj_raw<T> nj_load(const T* __restrict__ p, int n) {
+    if (n >= 4) return *reinterpret_cast<const t8_v4<T>*>(p);
     nj_raw<T> v = nj_raw<T>(0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 3; ++i)
         if (i < n) v[i] = p[i];
     return v;
 }
@@ -194,9 +188,9 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join(const NjArgs 
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            nf[i] = nj_load(f + r * a.ldf + c, a.vec, W - c);
-            if (x) nx[i] = nj_load(x + r * a.ldx + c, a.vec, W - c);
-            if (a.has_gate) ng[i] = nj_load(gate + gr * a.ldg + c, a.vec, W - c);
+            nf[i] = nj_load(f + r * a.ldf + c, W - c);
+            if (x) nx[i] = nj_load(x + r * a.ldx + c, W - c);
+            if (a.has_gate) ng[i] = nj_load(gate + gr * a.ldg + c, W - c);
         }
     };
     if (row < a.M) load(row, g);
@@ -220,7 +214,7 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join(const NjArgs 
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
             s[i] += m[i] * (v[i] * pg[i] + pb[i]);                            // (gain one, bias zero where there is none)
-            t8_store4(y + row * a.ldy + c, a.vec, W - c, s[i]);
+            t8_store4(y + row * a.ldy + c, W - c, s[i]);
         }
         if (!a.has_pre) continue;
         // (the second norm reads y before it is rounded to T)
@@ -232,7 +226,7 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join(const NjArgs 
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            t8_store4(h + row * a.ldh + c, a.vec, W - c, s[i] * qg[i] + qb[i]);
+            t8_store4(h + row * a.ldh + c, W - c, s[i] * qg[i] + qb[i]);
         }
     }
 }
@@ -272,9 +266,9 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            ny[i] = nj_load(gy + r * a.ldx + c, a.vec, W - c);
-            if (a.has_pre) nh[i] = nj_load(gh + r * a.ldf + c, a.vec, W - c);
-            if (a.has_gate) ng[i] = nj_load(gate + gr * a.ldg + c, a.vec, W - c);
+            ny[i] = nj_load(gy + r * a.ldx + c, W - c);
+            if (a.has_pre) nh[i] = nj_load(gh + r * a.ldf + c, W - c);
+            if (a.has_gate) ng[i] = nj_load(gate + gr * a.ldg + c, W - c);
             npc[i] = npe[i] = nqc[i] = nqe[i] = 0u;
             if (c < W) {
                 npc[i] = *reinterpret_cast<const unsigned*>(a.post_c + r * (32 * blocks) + c);
@@ -330,7 +324,7 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            if (dx) t8_store4(dx + r * a.ldy + c, a.vec, W - c, D[i]);
+            if (dx) t8_store4(dx + r * a.ldy + c, W - c, D[i]);
             T0[i] += D[i], T1[i] += D[i] * v[i];
             D[i] *= gt[i] * sc[i] * pg[i];
         }
@@ -338,9 +332,9 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            t8_store4(df + r * a.ldh + c, a.vec, W - c, D[i]);
+            t8_store4(df + r * a.ldh + c, W - c, D[i]);
             if (OWN && ends) {
-                t8_store4(dgate + gr * W + c, a.vec, W - c, (T1[i] * pg[i] + T0[i] * pb[i]) * sc[i]);
+                t8_store4(dgate + gr * W + c, W - c, (T1[i] * pg[i] + T0[i] * pb[i]) * sc[i]);
                 S1[i] += gt[i] * T1[i], S0[i] += gt[i] * T0[i];
                 T1[i] = T0[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
             }
@@ -427,6 +421,9 @@ __global__ void __launch_bounds__(1024) k_norm_join_params(const NjArgs a, int n
 
 // ---------------------------------------------------------------------------------------------------------------------------- launches
 #define NJ_MAX_W 4096
+#ifndef NJ_MOST
+#define NJ_MOST 512
+#endif
 // lanes of a row's team: two slots of four columns each, sixteen lanes at least
 static int nj_team(int W) { return W <= 128 ? 16 : W <= 256 ? 32 : W <= 512 ? 64 : W <= 2048 ? 256 : 512; }
 static int nj_teams(int W) { return W <= 2048 ? 256 / nj_team(W) : 1; }
@@ -442,7 +439,7 @@ static long nj_bwd_grid(long M, int W, long G, int* per_group) {
     *per_group = 0;
     if (G <= 0 || G > 2048 || G == M) {
         const long n = ((G > 2048 ? G : M) + teams - 1) / teams;
-        return n < 512 ? n : 512;
+        return n < NJ_MOST ? n : NJ_MOST;
     }
     const long each = (M / G + teams - 1) / teams, n = G < 512 ? 512 / G : 1;
     *per_group = (int)(each < n ? each : n);
@@ -478,13 +475,6 @@ static void nj_backward(const NjArgs& a, dim3 grid, hipStream_t st) {
     else if (W <= 2048) k_norm_join_bwd<T, 256, 2, OWN><<<grid, 256, 0, st>>>(a);
     else k_norm_join_bwd<T, 512, 2, OWN><<<grid, 512, 0, st>>>(a);
 }
-static int nj_vec(int W, size_t size, const void* const* p, const long* ld, int n) {
-    int ok = !(W & 3);
-    for (int i = 0; i < n; ++i)
-        if (p[i]) ok &= !((uintptr_t)p[i] & (4 * size - 1)) && !(ld[i] & 3);
-    return ok;
-}
-
 extern "C" int magnet_norm_join(const void* x, long ldx, const void* f, long ldf, int dtype, long M, int W, int layer, float eps, const float* post_g,
                                 const float* post_b, const float* pre_g, const float* pre_b, const void* gate, long ldg, long G, const float* scale_v,
                                 float scale, void* y, void* h, void* post_codes, void* post_bytes, float* post_rstd, void* pre_codes, void* pre_bytes,
@@ -494,16 +484,12 @@ extern "C" int magnet_norm_join(const void* x, long ldx, const void* f, long ldf
     if (!y || (post_b && !post_g) || (pre_b && !pre_g) || (pre_g && !h)) return -2;
     const int tape = post_codes != nullptr;
     if (tape && (!post_bytes || (post_g && !post_rstd) || (pre_g && (!pre_codes || !pre_bytes || !pre_rstd)))) return -2;
-    const size_t size = dtype == T8_F32 ? 4 : 2;
     NjArgs a = {};
     a.x = x, a.f = f, a.gate = gate, a.scale_v = scale_v, a.post_g = post_g, a.post_b = post_b, a.pre_g = pre_g, a.pre_b = pre_b, a.y = y, a.h = h;
     a.post_c = (unsigned char*)post_codes, a.post_e = (unsigned char*)post_bytes, a.pre_c = (unsigned char*)pre_codes, a.pre_e = (unsigned char*)pre_bytes;
     a.post_r = post_rstd, a.pre_r = pre_rstd, a.M = M, a.ldx = ldx, a.ldf = ldf, a.ldg = ldg, a.ldy = W, a.ldh = W;
     a.rows_per_gate = gate ? M / G : M, a.W = W, a.layer = layer, a.has_post = post_g != nullptr, a.has_pre = pre_g != nullptr, a.has_gate = gate != nullptr;
     a.tape = tape, a.scale = scale, a.eps = eps;
-    const void* p[] = {x, f, gate, y, h};
-    const long ld[] = {ldx, ldf, ldg, W, W};
-    a.vec = nj_vec(W, size, p, ld, 5);
     if (dtype == T8_F32) nj_forward<float>(a, (hipStream_t)stream);
     else nj_forward<__bf16>(a, (hipStream_t)stream);
     return (int)hipGetLastError();
@@ -516,9 +502,6 @@ extern "C" int magnet_norm_tape(const void* z, long ldz, int dtype, long M, int 
     NjArgs a = {};
     a.f = z, a.post_c = (unsigned char*)codes, a.post_e = (unsigned char*)bytes, a.post_r = rstd, a.M = M, a.ldf = ldz, a.rows_per_gate = M, a.W = W;
     a.layer = layer, a.has_post = 1, a.tape = 1, a.eps = eps;
-    const void* p[] = {z};
-    const long ld[] = {ldz};
-    a.vec = nj_vec(W, dtype == T8_F32 ? 4 : 2, p, ld, 1);
     if (dtype == T8_F32) nj_forward<float>(a, (hipStream_t)stream);
     else nj_forward<__bf16>(a, (hipStream_t)stream);
     return (int)hipGetLastError();
@@ -532,16 +515,12 @@ extern "C" int magnet_norm_join_bwd(const void* gy, long ldgy, const void* gh, l
     if (M < 1 || W < 1 || W > NJ_MAX_W || ldgy < W || (dtype != T8_F32 && dtype != T8_BF16) || !df || (gate && (G < 1 || M % G || ldg < W || !dgate)))
         return -2;
     if (!post_codes || !post_bytes || (post_g && !post_rstd) || (pre_g && (!gh || ldgh < W || !pre_codes || !pre_bytes || !pre_rstd))) return -2;
-    const size_t size = dtype == T8_F32 ? 4 : 2;
     NjArgs a = {};
     a.x = gy, a.f = gh, a.gate = gate, a.scale_v = scale_v, a.post_g = post_g, a.post_b = post_b, a.pre_g = pre_g, a.pre_b = pre_b, a.y = dx, a.h = df;
     a.post_c = (unsigned char*)post_codes, a.post_e = (unsigned char*)post_bytes, a.pre_c = (unsigned char*)pre_codes, a.pre_e = (unsigned char*)pre_bytes;
     a.post_r = (float*)post_rstd, a.pre_r = (float*)pre_rstd, a.dgate = dgate, a.part = workspace;
     a.M = M, a.ldx = ldgy, a.ldf = ldgh, a.ldg = ldg, a.ldy = W, a.ldh = W, a.rows_per_gate = gate ? M / G : M, a.W = W, a.layer = layer;
     a.has_post = post_g != nullptr, a.has_pre = pre_g != nullptr, a.has_gate = gate != nullptr, a.scale = scale;
-    const void* p[] = {gy, pre_g ? gh : nullptr, gate, dx, df, dgate};
-    const long ld[] = {ldgy, ldgh, ldg, W, W, W};
-    a.vec = nj_vec(W, size, p, ld, 6);
     const long grid = nj_bwd_grid(M, W, gate ? G : 0, &a.per_group);
     a.groups = gate ? G : 1;
     a.need_sums = a.per_group || d_scale || d_post_g || d_post_b || d_pre_g || d_pre_b;

@@ -20,36 +20,35 @@ typedef unsigned t8_u4 __attribute__((ext_vector_type(4)));
 enum { T8_SIGNED = 0, T8_RELU = 1 };
 enum { T8_F32 = 0, T8_BF16 = 1, T8_F16 = 2 };
 
-// four neighbouring values as fp32; vec: 4 sizeof(T)-byte aligned and all four exist, else one by one up to n (the rest zero)
+// four neighbouring values of any alignment (the hardware takes 16-byte accesses at 4-byte, 8-byte ones at 2-byte addresses)
 template <typename T>
-__device__ __forceinline__ t8_f4 t8_load4(const T* __restrict__ p, bool vec, int n) {
-    typedef T tv __attribute__((ext_vector_type(4)));
+using t8_v4 = T __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+// ... as fp32; of fewer than four (a row's end) the ones that are there, the rest zero
+template <typename T>
+__device__ __forceinline__ t8_f4 t8_load4(const T* __restrict__ p, int n) {
     t8_f4 v = {0.f, 0.f, 0.f, 0.f};
-    if (n <= 0) return v;
-    if (vec) {
-        const tv t = *reinterpret_cast<const tv*>(p);
+    if (n >= 4) {
+        const t8_v4<T> t = *reinterpret_cast<const t8_v4<T>*>(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = (float)t[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 3; ++i)
             if (i < n) v[i] = (float)p[i];
     }
     return v;
 }
 // ... and back, each value rounded to T once (to nearest, ties to even)
 template <typename T>
-__device__ __forceinline__ void t8_store4(T* __restrict__ p, bool vec, int n, const t8_f4& v) {
-    typedef T tv __attribute__((ext_vector_type(4)));
-    if (n <= 0) return;
-    if (vec) {
-        tv t;
+__device__ __forceinline__ void t8_store4(T* __restrict__ p, int n, const t8_f4& v) {
+    if (n >= 4) {
+        t8_v4<T> t;
 #pragma unroll
         for (int i = 0; i < 4; ++i) t[i] = (T)v[i];
-        *reinterpret_cast<tv*>(p) = t;
+        *reinterpret_cast<t8_v4<T>*>(p) = t;
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 3; ++i)
             if (i < n) p[i] = (T)v[i];
     }
 }

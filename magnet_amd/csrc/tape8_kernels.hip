@@ -23,7 +23,7 @@ struct T8Walk {                          // position (row, group of columns) of 
 };
 
 template <typename T, int KIND>
-__global__ void __launch_bounds__(256) k_tape8_pack(const T* __restrict__ x, long ldx, long M, int W, int vec, unsigned char* __restrict__ codes,
+__global__ void __launch_bounds__(256) k_tape8_pack(const T* __restrict__ x, long ldx, long M, int W, unsigned char* __restrict__ codes,
                                                     unsigned char* __restrict__ bytes) {
     const int blocks = (W + 31) / 32;
     T8Walk at((long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, blocks * (32 / T8_CPL));
@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(256) k_tape8_pack(const T* __restrict__ x, lon
 #pragma unroll
         for (int h = 0; h < T8_CPL / 4; ++h) {
             const int ch = c + 4 * h;
-            v[h] = t8_load4(x + at.row * ldx + ch, vec && ch < W, W - ch);
+            v[h] = t8_load4(x + at.row * ldx + ch, W - ch);
             top = max(top, t8_top4<KIND>(v[h]));
         }
         top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));      // quad_perm 1 0 3 2, 2 3 0 1
@@ -45,16 +45,32 @@ __global__ void __launch_bounds__(256) k_tape8_pack(const T* __restrict__ x, lon
     }
 }
 
-// (four columns per lane here: what it writes is four times what it reads, and a store instruction then covers a run of whole lines)
+// (as many columns per lane as make 16 bytes of the result: what it writes is two or four times what it reads, and a store instruction
+// then covers a run of whole lines)
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256) k_tape8_unpack(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ bytes, long M, int W,
-                                                      T* __restrict__ y, long ldy, int vec) {
+                                                      T* __restrict__ y, long ldy) {
+    constexpr int CPL = 16 / sizeof(T), LPB = 32 / CPL;                       // columns per lane, lanes per block
     const int blocks = (W + 31) / 32;
-    T8Walk at((long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, blocks * 8);
+    T8Walk at((long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, blocks * LPB);
     for (; at.row < M; at.next()) {
-        const int c = 4 * at.g;
-        const unsigned w = *reinterpret_cast<const unsigned*>(codes + at.row * (32 * blocks) + c);
-        t8_store4(y + at.row * ldy + c, vec && c < W, W - c, t8_decode4<KIND>(w, bytes[at.row * blocks + (at.g >> 3)]));
+        const int c = CPL * at.g;
+        const unsigned char* p = codes + at.row * (32 * blocks) + c;
+        const unsigned byte = bytes[at.row * blocks + at.g / LPB];
+        T* o = y + at.row * ldy + c;
+        if (CPL == 4) {
+            t8_store4(o, W - c, t8_decode4<KIND>(*reinterpret_cast<const unsigned*>(p), byte));
+        } else {
+            typedef T t8_v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+            const t8_u2 w = *reinterpret_cast<const t8_u2*>(p);
+            const t8_f4 u = t8_decode4<KIND>(w[0], byte), v = t8_decode4<KIND>(w[1], byte);
+            if (c + 8 <= W) {
+                *reinterpret_cast<t8_v8*>(o) = t8_v8{(T)u[0], (T)u[1], (T)u[2], (T)u[3], (T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+            } else {
+                t8_store4(o, W - c, u);
+                t8_store4(o + 4, W - c - 4, v);
+            }
+        }
     }
 }
 
@@ -63,27 +79,22 @@ static unsigned t8_grid(long M, int W, int lanes_per_block) {
     const long n = (M * ((W + 31) / 32) * lanes_per_block + 255) / 256;
     return (unsigned)(n < 1 ? 1 : n > (1l << 24) ? 1l << 24 : n);
 }
-// four values at once: the width, the row stride and the address are multiples of four values
-static int t8_vec(const void* p, long ld, int W, size_t size) { return !(W & 3) && !(ld & 3) && !((uintptr_t)p & (4 * size - 1)); }
-
 template <typename T>
 static int t8_pack_as(const void* x, long ldx, long M, int W, int kind, void* codes, void* bytes, hipStream_t st) {
-    const int vec = t8_vec(x, ldx, W, sizeof(T));
     const dim3 grid(t8_grid(M, W, 32 / T8_CPL));
     if (kind == T8_RELU)
-        k_tape8_pack<T, T8_RELU><<<grid, 256, 0, st>>>((const T*)x, ldx, M, W, vec, (unsigned char*)codes, (unsigned char*)bytes);
+        k_tape8_pack<T, T8_RELU><<<grid, 256, 0, st>>>((const T*)x, ldx, M, W, (unsigned char*)codes, (unsigned char*)bytes);
     else
-        k_tape8_pack<T, T8_SIGNED><<<grid, 256, 0, st>>>((const T*)x, ldx, M, W, vec, (unsigned char*)codes, (unsigned char*)bytes);
+        k_tape8_pack<T, T8_SIGNED><<<grid, 256, 0, st>>>((const T*)x, ldx, M, W, (unsigned char*)codes, (unsigned char*)bytes);
     return (int)hipGetLastError();
 }
 template <typename T>
 static int t8_unpack_as(const void* codes, const void* bytes, long M, int W, int kind, void* y, long ldy, hipStream_t st) {
-    const int vec = t8_vec(y, ldy, W, sizeof(T));
-    const dim3 grid(t8_grid(M, W, 8));
+    const dim3 grid(t8_grid(M, W, 32 * sizeof(T) / 16));
     if (kind == T8_RELU)
-        k_tape8_unpack<T, T8_RELU><<<grid, 256, 0, st>>>((const unsigned char*)codes, (const unsigned char*)bytes, M, W, (T*)y, ldy, vec);
+        k_tape8_unpack<T, T8_RELU><<<grid, 256, 0, st>>>((const unsigned char*)codes, (const unsigned char*)bytes, M, W, (T*)y, ldy);
     else
-        k_tape8_unpack<T, T8_SIGNED><<<grid, 256, 0, st>>>((const unsigned char*)codes, (const unsigned char*)bytes, M, W, (T*)y, ldy, vec);
+        k_tape8_unpack<T, T8_SIGNED><<<grid, 256, 0, st>>>((const unsigned char*)codes, (const unsigned char*)bytes, M, W, (T*)y, ldy);
     return (int)hipGetLastError();
 }
 

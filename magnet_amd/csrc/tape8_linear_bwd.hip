@@ -34,7 +34,7 @@ struct T8LinArgs {
     float* wpart;                        // [K blocks][gridDim.x][NP][KP] partial sums of dW
     float* bpart;                        // [gridDim.x][NP] partial sums of db
     long M, ldz, ldw, lddx;
-    int N, K, ldc, zvec, xvec, add_dx;   // zvec / xvec: dz / dx in 16-byte accesses; add_dx: dx += (a later block of N)
+    int N, K, ldc, exact, add_dx;        // exact: N = NP and K a multiple of KP; add_dx: dx += (a later block of N)
 };
 
 // exponent byte (1 .. 254) of a magnitude's bits; 0 for zero, subnormals and what is not finite
@@ -86,8 +86,10 @@ __device__ __forceinline__ void t8_put(void* base, unsigned off, const V& v) {
 }
 #define T8_UNIFORM(p) asm volatile("" : "+s"(p))
 
-// FULL: N = NP, K a multiple of KP, dz and dx in 16-byte accesses, one block of N - no lane ever looks at a column that is not there, and
-// addresses are a uniform base and one offset (the registers that bounds and addresses take are what decides between spilling and not)
+// FULL: at least 64 rows, N and K multiples of four, one block of N.  Addresses are then a uniform base and one offset per lane, and nothing is
+// loaded under a condition (the registers that bounds and addresses take are what decides between spilling and not): a lane whose
+// columns do not exist loads existing ones instead - of dz times a scale of zero, of the tape into columns of dx and dW that are not
+// written - and the last step takes the last R rows, those done already likewise.
 // 128 x 128 has eight waves, the smaller shapes four.  A wave's tiles are near square - 32 features of x by half the rows for dx, 32 features
 // of dz by 64 of x for dW - because what a tile needs from LDS is its two edges: 524 us at 2 097 152 rows, 537 with sixteen features by all
 // rows for each wave.  Behind Swish, where a step has half the rows, it is the other way round: 105 us against 118 at 262 144 rows.
@@ -125,7 +127,8 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     auto load = [&](long step) {
         if (FULL) {
             const long row = min(step * R, a.M - R);
-            const unsigned oz = ((unsigned)zr * (unsigned)a.ldz + zc) * 4u, oc = (unsigned)cr * (unsigned)a.ldc + cc, ob = (unsigned)cr * (unsigned)lb + cc / 32;
+            const int zcl = zc < a.N ? zc : 0, ccl = c_on ? cc : 0;
+            const unsigned oz = ((unsigned)zr * (unsigned)a.ldz + zcl) * 4u, oc = (unsigned)cr * (unsigned)a.ldc + ccl, ob = (unsigned)cr * (unsigned)lb + ccl / 32;
             const unsigned char *bc = a.codes + row * a.ldc + k0, *bb = a.bytes + row * lb + k0 / 32;
             T8_UNIFORM(bc);
             T8_UNIFORM(bb);
@@ -133,7 +136,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             for (int i = 0; i < NLD; ++i) {
                 const float* p = a.dz + (row + i * RPL) * a.ldz;
                 T8_UNIFORM(p);
-                dv[i] = t8_at<t8_f4>(p, oz);
+                dv[i] = t8_at<t8_v4<float>>(p, oz);
             }
             cv = t8_at<t8_cw>(bc, oc), bv = t8_at<unsigned char>(bb, ob);
             return;
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
             const long r = step * R + zr + i * RPL;
-            dv[i] = r < a.M ? t8_load4(a.dz + r * a.ldz + zc, a.zvec && zc < a.N, a.N - zc) : t8_f4{0.f, 0.f, 0.f, 0.f};
+            dv[i] = r < a.M ? t8_load4(a.dz + r * a.ldz + zc, a.N - zc) : t8_f4{0.f, 0.f, 0.f, 0.f};
         }
         const long r = step * R + cr;
         const bool on = c_on && r < a.M;
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     {
         auto w_at = [&](int b, int t, int j) -> float {
             const int n = 32 * t + 8 * q4 + j, k = k0 + kf + 16 * b + n16;
-            if (FULL) {
+            if (FULL && a.exact) {
                 const float* p = a.w + (32 * t + j) * a.ldw + k0 + kf + 16 * b;
                 T8_UNIFORM(p);
                 return t8_at<float>(p, ((unsigned)(8 * q4) * (unsigned)a.ldw + n16) * 4u);
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
-            const float G = FULL && zr + i * RPL < shift ? 0.f : t8_pow2(267 - ze);
+            const float G = FULL && (zr + i * RPL < shift || zc >= a.N) ? 0.f : t8_pow2(267 - ze);
             t8_u2 h, l;
             unsigned hw, lw;
             m = fmaxf(fmaxf(fmaxf(m, fabsf(dv[i][0])), fabsf(dv[i][1])), fmaxf(fabsf(dv[i][2]), fabsf(dv[i][3])));
@@ -334,11 +337,11 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                         if (FULL) {
                             float* o = bx + 16 * rb * a.lddx + 16 * b;
                             T8_UNIFORM(o);
-                            if (lr >= done) t8_put<t8_f4>(o, ox, v);
+                            if (lr >= done && k < a.K) t8_put<t8_v4<float>>(o, ox, v);
                         } else if (row0 + lr < a.M) {
                             float* o = a.dx + (row0 + lr) * a.lddx + k;
-                            if (a.add_dx) v += t8_load4(o, a.xvec && k < a.K, a.K - k);
-                            t8_store4(o, a.xvec && k < a.K, a.K - k, v);
+                            if (a.add_dx) v += t8_load4(o, a.K - k);
+                            t8_store4(o, a.K - k, v);
                         }
                     }
                 }
@@ -488,11 +491,10 @@ extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void
         a.dz = dz + n0, a.codes = (const unsigned char*)codes, a.bytes = (const unsigned char*)bytes, a.w = w + n0 * ldw, a.dx = dx;
         a.wpart = workspace, a.bpart = workspace + (size_t)grid.x * np * kp * kb;
         a.M = M, a.ldz = ldz, a.ldw = ldw, a.lddx = lddx, a.N = n, a.K = K, a.ldc = (K + 31) / 32 * 32;
-        a.zvec = !(n & 3) && !(ldz & 3) && !((uintptr_t)a.dz & 15);
-        a.xvec = !(K & 3) && !(lddx & 3) && !((uintptr_t)dx & 15);
+        a.exact = n == np && !(K % kp);
         a.add_dx = n0 > 0;
         // (32-bit byte offsets inside a step of 32 rows)
-        const bool full = M >= 64 && N == np && !(K % kp) && a.zvec && (a.xvec || !dx) && ldz < (1l << 24) && lddx < (1l << 24) && ldw < (1l << 24);
+        const bool full = M >= 64 && N <= T8_BLOCK && !(n & 3) && !(K & 3) && ldz < (1l << 24) && lddx < (1l << 24) && ldw < (1l << 24);
         if (full) t8_lin_shape<true>(a, np, kp, act, grid, st);
         else t8_lin_shape<false>(a, np, kp, act, grid, st);
         k_tape8_linear_sum<<<dim3((np * kp + 63) / 64, kb + 1), 1024, 0, st>>>(a.wpart, a.bpart, grid.x, np, kp, n, K, dW + n0 * lddw, lddw, db ? db + n0 : nullptr, accumulate);
