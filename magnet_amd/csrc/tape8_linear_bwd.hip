@@ -64,6 +64,8 @@ __device__ __forceinline__ float t8_swish(float v, float& d) {
 #define T8_WAVES(NP, KP) ((NP) == 128 && (KP) == 128 ? 8 : 4)
 #define T8_ROWS(NP, KP, ACT) ((NP) == (KP) && (ACT) != ACT_SWISH ? 64 : 32)      // rows of a step
 #define T8_TILE(NP, KP, ACT) ((NP) == 128 && (KP) == 128 && (ACT) == ACT_SWISH ? 1 : 2)       // blocks of 16 features of a wave's tiles
+#define T8_FOLD 8                        // steps whose products are added up in a row before they join the sums so far: a chain of additions in fp32
+                                         // is off by its length (2 097 152 rows: 1.7e-6 of dW in one chain per workgroup)
 #define T8_ZROOM 3                       // binades of dz and of the tape's bytes that may still come before the scale has to change
 #define T8_XROOM 2
 template <int NP, int KP, int XPL, int R, int ACT>
@@ -167,16 +169,23 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             }
             return n < a.N && k < a.K ? a.w[n * a.ldw + k] : 0.f;
         };
-        unsigned top = 0;
+        float wv[NBK][NT][8];                                                 // (the sums' registers are not in use yet)
 #pragma unroll
         for (int b = 0; b < NBK; ++b)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) top = max(top, t8_expo(w_at(b, t, j)));
+                for (int j = 0; j < 8; ++j) wv[b][t][j] = w_at(b, t, j);
+        unsigned et = 0;
 #pragma unroll
-        for (int o = 32; o; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
-        we = max(__builtin_amdgcn_readfirstlane((int)top), 14);
+        for (int b = 0; b < NBK; ++b)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) et = max(et, t8_expo(wv[b][t][j]));
+#pragma unroll
+        for (int o = 32; o; o >>= 1) et = max(et, (unsigned)__shfl_xor((int)et, o));
+        we = max(__builtin_amdgcn_readfirstlane((int)et), 14);
         const float s = t8_pow2(267 - we);
 #pragma unroll
         for (int b = 0; b < NBK; ++b)
@@ -186,7 +195,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     unsigned hw, lw;
-                    split_f16_prod(w_at(b, t, 2 * j), s, w_at(b, t, 2 * j + 1), s, hw, lw);
+                    split_f16_prod(wv[b][t][2 * j], s, wv[b][t][2 * j + 1], s, hw, lw);
                     h[j] = hw, l[j] = lw;
                 }
                 wh[b][t] = __builtin_bit_cast(t8_h8, h), wl[b][t] = __builtin_bit_cast(t8_h8, l);
@@ -271,109 +280,124 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             xe = __builtin_amdgcn_readfirstlane((int)mx > xe ? (int)mx + T8_XROOM : xe);
             if (tid < 2) flag[tid] = 0u;                                      // (everybody has read the flag that ended the last stretch)
         }
-        f32x4 accw[NBN][KB];
+        f32x4 accs[NBN][KB];                                                  // the stretch's sums: T8_FOLD steps at a time
 #pragma unroll
         for (int b = 0; b < NBN; ++b)
 #pragma unroll
-            for (int x = 0; x < KB; ++x) accw[b][x] = f32x4{0.f, 0.f, 0.f, 0.f};
-        // (a stretch's first step is what its bounds were made of: nothing to ask - and what is not finite would ask for more for ever)
-        for (bool fresh = true; step < nsteps; step += gridDim.x, ++it, fresh = false) {
-        Step& B = sb[it & 1];
-        if (FULL) shift = (int)(step * R - min(step * R, a.M - R));
-        const bool over = stage(B);
-        if (!fresh && __any(over) && lane == 0) flag[it & 1] = 1u;
-        wg_barrier();
-        if (!fresh && __builtin_amdgcn_readfirstlane((int)flag[it & 1])) break;     // (the same for every wave)
+            for (int x = 0; x < KB; ++x) accs[b][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        bool fresh = true, same = true;
+        while (same && step < nsteps) {
+            f32x4 accw[NBN][KB];
 #pragma unroll
-        for (int i = 0; i < NLD; ++i)
-            if (!FULL || zr + i * RPL >= shift) bsum += dv[i];
-        const long row0 = FULL ? min(step * R, a.M - R) : step * R;
-        const int done = shift;
-        asm volatile("" ::: "memory");
-        load(min(step + (long)gridDim.x, nsteps - 1));                        // (past the last step: rows that nobody uses)
-        asm volatile("" ::: "memory");
-        // ---- dx^T: acc[b][rb] = features kf + 16 b .. of rows wr + 16 (rp + rb) ..
+            for (int b = 0; b < NBN; ++b)
 #pragma unroll
-        for (int rp = 0; rp < RBS; rp += RB) {
-            f32x4 acc[NBK][RB];
-#pragma unroll
-            for (int b = 0; b < NBK; ++b)
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) acc[b][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const t8_h8 zh = *reinterpret_cast<const t8_h8*>(&B.z[0][wr + 16 * (rp + rb) + n16][32 * t + 8 * q4]);
-                    const t8_h8 zl = *reinterpret_cast<const t8_h8*>(&B.z[1][wr + 16 * (rp + rb) + n16][32 * t + 8 * q4]);
-#pragma unroll
-                    for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl[b][t], zh, acc[b][rb], 0, 0, 0);
-#pragma unroll
-                    for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zl, acc[b][rb], 0, 0, 0);
-#pragma unroll
-                    for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zh, acc[b][rb], 0, 0, 0);
+                for (int x = 0; x < KB; ++x) accw[b][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+            // (a stretch's first step is what its bounds were made of: nothing to ask - and what is not finite would ask for more for ever)
+            for (int k = 0; k < T8_FOLD && step < nsteps; ++k, step += gridDim.x, ++it, fresh = false) {
+                Step& B = sb[it & 1];
+                if (FULL) shift = (int)(step * R - min(step * R, a.M - R));
+                const bool over = stage(B);
+                if (!fresh && __any(over) && lane == 0) flag[it & 1] = 1u;
+                wg_barrier();
+                if (!fresh && __builtin_amdgcn_readfirstlane((int)flag[it & 1])) {          // (the same for every wave)
+                    same = false;
+                    break;
                 }
-            __builtin_amdgcn_sched_barrier(0);                                // (without these the reads of all parts move up and the registers run out)
-            // dx = act'(v) (dz W): lane = row n16 of the block of rows, features 4 q4 .. + 3 of the block of features
-            if (a.dx) {
-                const int e = we + ze - 280;
-                float* const bx = a.dx + (row0 + wr + 16 * rp) * a.lddx + k0 + kf;
-                const unsigned ox = ((unsigned)n16 * (unsigned)a.lddx + 4 * q4) * 4u;
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const int lr = wr + 16 * (rp + rb) + n16;                 // row of the step
+                for (int i = 0; i < NLD; ++i)
+                    if (!FULL || zr + i * RPL >= shift) bsum += dv[i];
+                const long row0 = FULL ? min(step * R, a.M - R) : step * R;
+                const int done = shift;
+                asm volatile("" ::: "memory");
+                load(min(step + (long)gridDim.x, nsteps - 1));                        // (past the last step: rows that nobody uses)
+                asm volatile("" ::: "memory");
+                // ---- dx^T: acc[b][rb] = features kf + 16 b .. of rows wr + 16 (rp + rb) ..
 #pragma unroll
-                    for (int b = 0; b < NBK; ++b) {
-                        const int f = kf + 16 * b + 4 * q4, k = k0 + f;
-                        t8_f4 v;
+                for (int rp = 0; rp < RBS; rp += RB) {
+                    f32x4 acc[NBK][RB];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(acc[b][rb][i], e);
-                        if (ACT == ACT_RELU) {
-                            const unsigned w = B.c[lr][f / 4];
+                    for (int b = 0; b < NBK; ++b)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = (w >> (8 * i)) & 0xFFu ? v[i] : 0.f;
+                        for (int rb = 0; rb < RB; ++rb) acc[b][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) {
+                            const t8_h8 zh = *reinterpret_cast<const t8_h8*>(&B.z[0][wr + 16 * (rp + rb) + n16][32 * t + 8 * q4]);
+                            const t8_h8 zl = *reinterpret_cast<const t8_h8*>(&B.z[1][wr + 16 * (rp + rb) + n16][32 * t + 8 * q4]);
+#pragma unroll
+                            for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl[b][t], zh, acc[b][rb], 0, 0, 0);
+#pragma unroll
+                            for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zl, acc[b][rb], 0, 0, 0);
+#pragma unroll
+                            for (int b = 0; b < NBK; ++b) acc[b][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[b][t], zh, acc[b][rb], 0, 0, 0);
                         }
-                        if (ACT == ACT_SWISH) v *= *reinterpret_cast<const t8_f4*>(&B.d[lr][f]);
-                        if (FULL) {
-                            float* o = bx + 16 * rb * a.lddx + 16 * b;
-                            T8_UNIFORM(o);
-                            if (lr >= done && k < a.K) t8_put<t8_v4<float>>(o, ox, v);
-                        } else if (row0 + lr < a.M) {
-                            float* o = a.dx + (row0 + lr) * a.lddx + k;
-                            if (a.add_dx) v += t8_load4(o, a.K - k);
-                            t8_store4(o, a.K - k, v);
+                    __builtin_amdgcn_sched_barrier(0);                                // (without these the reads of all parts move up and the registers run out)
+                    // dx = act'(v) (dz W): lane = row n16 of the block of rows, features 4 q4 .. + 3 of the block of features
+                    if (a.dx) {
+                        const int e = we + ze - 280;
+                        float* const bx = a.dx + (row0 + wr + 16 * rp) * a.lddx + k0 + kf;
+                        const unsigned ox = ((unsigned)n16 * (unsigned)a.lddx + 4 * q4) * 4u;
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) {
+                            const int lr = wr + 16 * (rp + rb) + n16;                 // row of the step
+#pragma unroll
+                            for (int b = 0; b < NBK; ++b) {
+                                const int f = kf + 16 * b + 4 * q4, k = k0 + f;
+                                t8_f4 v;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(acc[b][rb][i], e);
+                                if (ACT == ACT_RELU) {
+                                    const unsigned w = B.c[lr][f / 4];
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) v[i] = (w >> (8 * i)) & 0xFFu ? v[i] : 0.f;
+                                }
+                                if (ACT == ACT_SWISH) v *= *reinterpret_cast<const t8_f4*>(&B.d[lr][f]);
+                                if (FULL) {
+                                    float* o = bx + 16 * rb * a.lddx + 16 * b;
+                                    T8_UNIFORM(o);
+                                    if (lr >= done && k < a.K) t8_put<t8_v4<float>>(o, ox, v);
+                                } else if (row0 + lr < a.M) {
+                                    float* o = a.dx + (row0 + lr) * a.lddx + k;
+                                    if (a.add_dx) v += t8_load4(o, a.K - k);
+                                    t8_store4(o, a.K - k, v);
+                                }
+                            }
                         }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // ---- dW += dz^T x, 32 rows at a time (k group q4: rows 4 q4 .. + 3 and 16 + 4 q4 .. + 3 of both operands)
+#pragma unroll
+                for (int r32 = 0; r32 < R; r32 += 32) {
+                    const int r0 = r32 + 4 * q4 + (n16 >> 2), c0 = 4 * (n16 & 3);
+                    t8_h8 ah[NBN], al[NBN];
+#pragma unroll
+                    for (int b = 0; b < NBN; ++b) {
+                        const int f = nf + 16 * b + c0;
+                        ah[b] = t8_join(t8_tr(&B.z[0][r0][f]), t8_tr(&B.z[0][16 + r0][f]));
+                        al[b] = t8_join(t8_tr(&B.z[1][r0][f]), t8_tr(&B.z[1][16 + r0][f]));
+                    }
+#pragma unroll
+                    for (int x = 0; x < KB; ++x) {
+                        const int f = xf + 16 * x + c0;
+                        const t8_h8 xh = t8_join(t8_tr(&B.x[0][r0][f]), t8_tr(&B.x[0][16 + r0][f]));
+                        if (XPL == 2) {
+                            const t8_h8 xl = t8_join(t8_tr(&B.x[XPL - 1][r0][f]), t8_tr(&B.x[XPL - 1][16 + r0][f]));
+#pragma unroll
+                            for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b], xl, accw[b][x], 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[b], xh, accw[b][x], 0, 0, 0);
+#pragma unroll
+                        for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b], xh, accw[b][x], 0, 0, 0);
                     }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // ---- dW += dz^T x, 32 rows at a time (k group q4: rows 4 q4 .. + 3 and 16 + 4 q4 .. + 3 of both operands)
 #pragma unroll
-        for (int r32 = 0; r32 < R; r32 += 32) {
-            const int r0 = r32 + 4 * q4 + (n16 >> 2), c0 = 4 * (n16 & 3);
-            t8_h8 ah[NBN], al[NBN];
+            for (int b = 0; b < NBN; ++b)
 #pragma unroll
-            for (int b = 0; b < NBN; ++b) {
-                const int f = nf + 16 * b + c0;
-                ah[b] = t8_join(t8_tr(&B.z[0][r0][f]), t8_tr(&B.z[0][16 + r0][f]));
-                al[b] = t8_join(t8_tr(&B.z[1][r0][f]), t8_tr(&B.z[1][16 + r0][f]));
-            }
-#pragma unroll
-            for (int x = 0; x < KB; ++x) {
-                const int f = xf + 16 * x + c0;
-                const t8_h8 xh = t8_join(t8_tr(&B.x[0][r0][f]), t8_tr(&B.x[0][16 + r0][f]));
-                if (XPL == 2) {
-                    const t8_h8 xl = t8_join(t8_tr(&B.x[XPL - 1][r0][f]), t8_tr(&B.x[XPL - 1][16 + r0][f]));
-#pragma unroll
-                    for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b], xl, accw[b][x], 0, 0, 0);
-                }
-#pragma unroll
-                for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[b], xh, accw[b][x], 0, 0, 0);
-#pragma unroll
-                for (int b = 0; b < NBN; ++b) accw[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b], xh, accw[b][x], 0, 0, 0);
-            }
-        }
+                for (int x = 0; x < KB; ++x) accs[b][x] += accw[b][x];
         }
         // ---- the stretch's part of the workgroup's sums: C/D row 4 q4 + i = feature of dz, column n16 = feature of x
         // (the base hidden: 32 addresses would be kept in registers across the loop)
@@ -387,7 +411,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                     for (int i = 0; i < 4; ++i) {
                         float* o = wout + (nf + 16 * b + i) * KP + xf + 16 * x;
                         T8_UNIFORM(o);
-                        const float v = __builtin_amdgcn_ldexpf(accw[b][x][i], ze + xe - 272);
+                        const float v = __builtin_amdgcn_ldexpf(accs[b][x][i], ze + xe - 272);
                         t8_put<float>(o, ol, add ? t8_at<float>(o, ol) + v : v);
                     }
         };
