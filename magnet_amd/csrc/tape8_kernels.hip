@@ -74,10 +74,11 @@ __global__ void __launch_bounds__(256) k_tape8_unpack(const unsigned char* __res
     }
 }
 
-// one pass of every lane, up to the largest grid: a fixed number of workgroups that walk the array was 10 % slower at 2 097 152 x 128
+// one pass of every lane (up to a grid that still counts its lanes in 32 bits): a fixed number of workgroups that walk the array was 10 %
+// slower at 2 097 152 x 128
 static unsigned t8_grid(long M, int W, int lanes_per_block) {
     const long n = (M * ((W + 31) / 32) * lanes_per_block + 255) / 256;
-    return (unsigned)(n < 1 ? 1 : n > (1l << 24) ? 1l << 24 : n);
+    return (unsigned)(n < 1 ? 1 : n > (1l << 23) ? 1l << 23 : n);
 }
 template <typename T>
 static int t8_pack_as(const void* x, long ldx, long M, int W, int kind, void* codes, void* bytes, hipStream_t st) {

@@ -974,6 +974,8 @@ def tape8_linear_bwd(dz, tape: Tape8, w, act="none", *, need_dx=True, dx=None, d
     for o, name, shape in ((dx, "dx", (M, K)), (dW, "dW", (N, K)), (db, "db", (N,))):
         if o is not None and _overlap(_out_matrix(o, name, torch.float32, shape, None), dz):
             raise ValueError(f"magnet_amd: {name} must not overlap dz")
+        if o is not None and _overlap(o, w):
+            raise ValueError(f"magnet_amd: {name} must not overlap w")
     _on_device(dz, tape, w, dx, dW, db)
     dev = dz.device
     if need_dx and dx is None:

@@ -77,6 +77,8 @@ def test_linear_bwd_refusals():
     big = torch.randn(6, 80)
     with pytest.raises(ValueError, match="overlap"):
         go(big[:, 20:60], tape(6, 40), torch.randn(40, 40), dx=big[:, :40])
+    with pytest.raises(ValueError, match="overlap"):
+        go(dz, tape(6, 40), w, dW=w)
 
 
 def test_norm_join_refusals():

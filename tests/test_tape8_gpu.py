@@ -257,6 +257,50 @@ def test_linear_bwd_outputs_strides_and_accumulate():
     assert bool((a == 2.0).all()) and bool((b == 3.0).all())
 
 
+def test_linear_bwd_one_buffer_for_several_gradients():
+    """dW and db inside wider buffers, N in two blocks of 128: neighbours are left alone"""
+    from magnet_amd import ops
+    dz, t, w = linear_case(500, 150, 70, "none", seed=12)
+    want = ops.tape8_linear_bwd(dz, t, w)
+    flat = torch.full((150, 90), 4.0, device="cuda")
+    tail = torch.full((160,), 4.0, device="cuda")
+    dx, dW, db = ops.tape8_linear_bwd(dz, t, w, dW=flat[:, 7:77], db=tail[5:155])
+    assert torch.equal(dx, want[0]) and torch.equal(flat[:, 7:77], want[1]) and torch.equal(tail[5:155], want[2])
+    assert bool((flat[:, :7] == 4).all()) and bool((flat[:, 77:] == 4).all()) and bool((tail[:5] == 4).all()) and bool((tail[155:] == 4).all())
+
+
+def test_offsets_beyond_32_bits():
+    """17 000 000 rows of 128: the tape's offsets pass 2^31 bytes, the gradients' 2^32; the ends give what they give alone"""
+    from magnet_amd import ops
+    M, W, tail = 17_000_000, 128, 512
+    x = torch.randn(4096, W, device="cuda", dtype=torch.bfloat16).repeat((M + 4095) // 4096, 1)[:M]
+    x[-tail:] = torch.randn(tail, W, device="cuda").bfloat16()
+    t = ops.tape8_pack(x, "relu")
+    end = ops.tape8_pack(x[-tail:].clone(), "relu")
+    assert torch.equal(t.codes[-tail:], end.codes) and torch.equal(t.bytes[-tail:], end.bytes)
+    assert torch.equal(ops.tape8_unpack(t, torch.bfloat16)[-tail:], ops.tape8_unpack(end, torch.bfloat16))
+    del x
+    dz = torch.zeros(M, W, device="cuda")
+    dz[-tail:] = torch.randn(tail, W, device="cuda") * 1e-6
+    w = torch.randn(W, W, device="cuda") / 11
+    dx, dW, db = ops.tape8_linear_bwd(dz, t, w, "relu")
+    want, bound = linear_ref(dz[-tail:], end, w, "relu")
+    for g, r, b in zip((dx[-tail:], dW, db), want, bound):
+        assert float(((g.double() - r).abs() - b).max()) <= 0
+    assert not dx[:-tail].any()
+    del dx, t
+    z = torch.zeros(M, W, device="cuda")
+    z[-tail:] = torch.randn(tail, W, device="cuda")
+    one = (torch.ones(W, device="cuda"), None)
+    r = ops.norm_join(dz, z, post=one, tape=True)
+    e = ops.norm_join(dz[-tail:].clone(), z[-tail:].clone(), post=one, tape=True)
+    assert torch.equal(r.y[-tail:], e.y) and torch.equal(r.post_tape.codes[-tail:], e.post_tape.codes) and torch.equal(r.post_rstd[-tail:], e.post_rstd)
+    del r.y
+    g = ops.norm_join_bwd(z, post_tape=r.post_tape, post_rstd=r.post_rstd, post=one)
+    ge = ops.norm_join_bwd(z[-tail:].clone(), post_tape=e.post_tape, post_rstd=e.post_rstd, post=one)
+    assert torch.equal(g.f[-tail:], ge.f) and torch.equal(g.x[-tail:], ge.x)
+
+
 # ------------------------------------------------------------------------------------------------------ norms around a residual block
 EPS = 1e-5
 
@@ -627,6 +671,43 @@ def test_magnet_gnn_trains_with_the_tape_in_8_bits(teacher_forcing):
             continue
         off = float((got[1][1][n] - g).norm() / g.norm()) if float(g.norm()) else 0.0
         assert off <= 0.05, (n, off)
+
+
+def test_a_captured_training_step_with_the_tape_in_8_bits():
+    """graphs.TrainStepGraph over a model that trains with ``tape8``: the replays' losses and parameters are those of the eager steps"""
+    from magnet_amd.graphs import TrainStepGraph
+    from magnet_amd.models.factory import FACTORY
+    from oracle import models as O
+    from oracle.weightgen import fill_state_dict
+    from tests.helpers import load_case
+    name, hp, salt, batch, d = load_case("magnet_gnn_tiny")
+    hp.tape8 = True
+    hp.teacher_forcing = True
+    oracle = O.build(name, hp)
+    fill_state_dict(oracle, salt)
+    cb = {k: v.cuda() for k, v in batch.items()}
+    runs = []
+    for captured in (False, True):
+        model = FACTORY[name](hp)
+        model.load_state_dict(oracle.state_dict())
+        model = model.cuda().train()
+        opt = model.configure_optimizers()["optimizer"]
+        step = TrainStepGraph(model, opt) if captured else None
+        torch.manual_seed(3)
+        losses = []
+        for _ in range(5):
+            if captured:
+                losses.append(float(step(cb).detach()))
+            else:
+                opt.zero_grad()
+                loss = model.training_step(cb, 0)
+                loss.backward()
+                opt.step()
+                losses.append(float(loss.detach()))
+        runs.append((losses, [p.detach().clone() for p in model.parameters()]))
+        assert not captured or (step.replays == 5 and step.eager_steps == 0)
+    assert runs[0][0] == runs[1][0]
+    assert all(torch.equal(a, b) for a, b in zip(runs[0][1], runs[1][1]))
 
 
 # ------------------------------------------------------------------------------------------------------- together, streams, graphs
