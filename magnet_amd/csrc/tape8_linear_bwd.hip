@@ -2,9 +2,12 @@
 //     x  = act(v)   v = the tape's value: the activated input itself (none, relu) or Swish's argument (swish)
 //     dx [M][K] = act'(v) (dz W)        dW [N][K] (+)= dz^T x        db [N] (+)= column sums of dz
 // What has to move is dz in, dx out and 33/32 bytes a value of the tape: 1156 bytes a row at N = K = 128, where fp32 activations make it
-// 1536 (linear_bwd.hip).
+// 1536 (linear_bwd.hip).  Measured: 2 097 152 rows of 128 x 128 behind a ReLU 522 us (4.6 TB/s; a large copy reaches 4.9; the kernel
+// that reads fp32 activations 657 on the same box), 218 453 rows of 64 x 64 30 us, 262 144 rows of 128 x 128 behind Swish 105 us (20 of
+// them to start up and to add the partial sums; the exponentials, the second plane and the third product take turns with the loads: a
+// SIMD runs its vector and its matrix instructions at the sum of their times).
 //
-// A workgroup of four waves takes steps of 32 or 64 rows of one block of at most 128 x 128 of W.  dz is split once into two fp16 planes
+// A workgroup of four or eight waves takes steps of 32 or 64 rows of one block of at most 128 x 128 of W.  dz is split once into two fp16 planes
 // (h + l, 22 bits), the tape's codes need one plane - a code has 8 bits, fp16 holds code times a power of two exactly - (two behind
 // Swish), and both meet as 16 x 16 x 32 matrix products through LDS:
 //   dx^T = W^T dz^T   A = the wave's features of W^T, two planes kept in registers; B = rows of the dz image; products hh + hl + lh
@@ -16,7 +19,8 @@
 // met, of dz and of the tape's bytes, and stages everything times the power of two that puts the bound near the top of the range.  A lane
 // that meets more raises a flag with its write; behind the barrier that the step has anyway all waves see it, add their sums so far to the
 // workgroup's partial sums in memory and begin again under a new bound (with a few binades to spare): rare after the first step, and
-// nobody waits for a maximum otherwise.  (Scaling the sums in registers instead costs a second set of them: measured as spills.)  Rows 2^-24 below the largest so far start to lose bits, of a share that small of the sums.  A wave scales its part of W likewise.
+// nobody waits for a maximum otherwise.  (Scaling the sums in registers instead costs a second set of them: measured as spills.)  Rows
+// 2^-24 below the largest so far start to lose bits, of a share that small of the sums.  A wave scales its part of W likewise.
 #include "common.cuh"
 #include "split_single.cuh"
 #include "tape8.cuh"
@@ -62,7 +66,9 @@ __device__ __forceinline__ float t8_swish(float v, float& d) {
 }
 
 #define T8_WAVES(NP, KP) ((NP) == 128 && (KP) == 128 ? 8 : 4)
-#define T8_ROWS(NP, KP, ACT) ((NP) == (KP) && (ACT) != ACT_SWISH ? 64 : 32)      // rows of a step
+// rows of a step: 64 where two steps in LDS leave room for what a CU can hold in registers anyway (128 x 128: 539 us against 564 with 32 at
+// 2 097 152 rows; 64 x 64: 34 against 38 at 218 453); 32 for the mixed shapes (two workgroups a CU) and behind Swish (two planes)
+#define T8_ROWS(NP, KP, ACT) ((NP) == (KP) && (ACT) != ACT_SWISH ? 64 : 32)
 #define T8_TILE(NP, KP, ACT) ((NP) == 128 && (KP) == 128 && (ACT) == ACT_SWISH ? 1 : 2)       // blocks of 16 features of a wave's tiles
 #define T8_FOLD 8                        // steps whose products are added up in a row before they join the sums so far: a chain of additions in fp32
                                          // is off by its length (2 097 152 rows: 1.7e-6 of dW in one chain per workgroup)
