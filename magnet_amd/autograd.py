@@ -91,14 +91,15 @@ class tape8:
 
     def __init__(self, on=True):
         self.on = bool(on)
+        self.prev = []
 
     def __enter__(self):
-        self.prev = _TAPE8["on"]
+        self.prev.append(_TAPE8["on"])
         _TAPE8["on"] = self.on
         return self
 
     def __exit__(self, *exc):
-        _TAPE8["on"] = self.prev
+        _TAPE8["on"] = self.prev.pop()
         return False
 
 

@@ -140,7 +140,7 @@ class _RolloutScope:
         self.parts = (deferred_weight_checks(), model._guard.armed())
         if torch.is_grad_enabled() and model.training:      # a training step: loss.backward() follows (autograd.accumulate_param_grads)
             from ..autograd import accumulate_param_grads, tape8
-            self.parts += (accumulate_param_grads(), tape8(model.tape8))
+            self.parts += (accumulate_param_grads(), *([tape8()] if model.tape8 else []))      # (else as the caller has it)
 
     def __enter__(self):
         for p in self.parts:

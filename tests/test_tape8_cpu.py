@@ -135,3 +135,29 @@ def test_c_entries_refuse():
     assert L.magnet_tape8_linear_bwd_workspace(long(100), long(128), long(128), C.byref(n)) == 0 and n.value == 4 * (128 * 128 + 128)
     assert L.magnet_norm_join_bwd_workspace(long(100), long(128), long(3), C.byref(n)) == -2      # 3 gates for 100 rows
     assert L.magnet_norm_join_bwd_workspace(long(100), long(4097), long(0), C.byref(n)) == -2
+
+
+def test_the_context_nests_and_the_caller_s_stays():
+    """one context object entered twice restores what was; a model without ``tape8`` trains as the surrounding context says, one with it
+    in 8 bits"""
+    import contextlib
+    import types
+    from magnet_amd import autograd as AG
+    from magnet_amd.models.magnet_common import _RolloutScope
+    both = AG.tape8()
+    with both:
+        with both:
+            assert AG._TAPE8["on"]
+        assert AG._TAPE8["on"]
+        with AG.tape8(False):
+            assert not AG._TAPE8["on"]
+        assert AG._TAPE8["on"]
+    assert not AG._TAPE8["on"]
+    for outer in (False, True):
+        for own in (False, True):
+            model = types.SimpleNamespace(training=True, tape8=own, _guard=types.SimpleNamespace(armed=contextlib.nullcontext))
+            with AG.tape8(outer):
+                with _RolloutScope(model):
+                    assert AG._TAPE8["on"] is (outer or own)
+                assert AG._TAPE8["on"] is outer
+            assert not AG._TAPE8["on"]
