@@ -203,13 +203,14 @@ def _recompute_tape(M, kts, pk, nl, x0, X, zL, K0, x0_skip=0):
 _MEM = {"t": -1.0, "dev": None, "free": 0, "total": 1, "granted": 0}
 
 
-def _keep_tape(nbytes, dev):
+def _keep_tape(nbytes, dev, passing=0):
     """does the tape of one chain stay in memory from the forward to the backward?  MAGNET_KEEP_TAPE = 1 / 0 / auto (default): yes while
     it takes less than a quarter of what is still free and the device stays below 70 % full (MAGNET_TAPE_CAP) - later calls of a long rollout then fall
     back to recomputing by themselves.  "Free" is what the DEVICE reports (other processes, RCCL buffers, captured graphs' pools count)
     plus what torch's allocator holds in reserve; the figures are refreshed at most every 50 ms - a training step at the reference's
     batch sizes asks ~100 times and torch.cuda.memory_stats costs 0.1 ms a call (a fifth of such a step) - and the bytes granted since
-    the last refresh are subtracted."""
+    the last refresh are subtracted.  ``passing``: bytes that are needed on the way only (fp32 rows that go onto an 8-bit tape and are let go):
+    they must fit into half of what is free."""
     import os
     import time
     mode = os.environ.get("MAGNET_KEEP_TAPE", "auto")
@@ -222,7 +223,7 @@ def _keep_tape(nbytes, dev):
                     free=free_dev + torch.cuda.memory_reserved(dev) - torch.cuda.memory_allocated(dev))
     free = _MEM["free"] - _MEM["granted"]
     used = _MEM["total"] - free
-    ok = nbytes < 0.25 * free and used + nbytes < float(os.environ.get("MAGNET_TAPE_CAP", "0.7")) * _MEM["total"]
+    ok = nbytes < 0.25 * free and passing < 0.5 * free and used + nbytes < float(os.environ.get("MAGNET_TAPE_CAP", "0.7")) * _MEM["total"]
     if ok:
         _MEM["granted"] += nbytes
     return ok
@@ -417,7 +418,8 @@ class _Mlp(torch.autograd.Function):
             m.x0_dense = _x0_not_needed(m, srcs, m.M, np0, fk)        # the decision travels with the tape (not re-derived from the
             x0_free = m.x0_dense is not None                          # environment in the backward)
             K0t = 0 if x0_free else K0
-        if wants_tape and _keep_tape(m.M * (4 * K0t + ((nl - 1) * pk.ht * 32 + pk.ot * 32) * (33 / 32 if m.tape8 else 4)), y.device):
+        vals = m.M * ((nl - 1) * pk.ht * 32 + pk.ot * 32)
+        if wants_tape and _keep_tape(4 * m.M * K0t + vals * (33 / 32 if m.tape8 else 4), y.device, 4 * vals if m.tape8 else 0):
             new = lambda w: torch.empty(m.M, w, device=y.device, dtype=torch.float32)  # noqa: E731
             tape = (new(K0t), *[new(pk.ht * 32) for _ in range(nl - 1)], *([new(pk.ot * 32)] if pk.ln is not None else []))
             seg = dict(seg, x0_out=None if x0_free else tape[0], hid=list(tape[1:nl]) + [tape[nl] if pk.ln is not None else None],

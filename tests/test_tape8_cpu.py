@@ -161,3 +161,16 @@ def test_the_context_nests_and_the_caller_s_stays():
                     assert AG._TAPE8["on"] is (outer or own)
                 assert AG._TAPE8["on"] is outer
             assert not AG._TAPE8["on"]
+
+
+def test_a_tape_is_kept_only_where_the_rows_that_become_it_fit(monkeypatch):
+    """the chain's launch writes fp32 rows before they are packed: four times the tape, in memory for a moment"""
+    from magnet_amd import autograd as AG
+    monkeypatch.delenv("MAGNET_KEEP_TAPE", raising=False)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda dev: (100 << 30, 288 << 30))
+    monkeypatch.setattr(torch.cuda, "memory_reserved", lambda dev: 0)
+    monkeypatch.setattr(torch.cuda, "memory_allocated", lambda dev: 0)
+    monkeypatch.setenv("MAGNET_TAPE_CAP", "1.0")
+    for passing, kept in ((0, True), (40 << 30, True), (60 << 30, False)):
+        monkeypatch.setattr(AG, "_MEM", dict(dev=None, t=0.0, total=0, free=0, granted=0))
+        assert AG._keep_tape(15 << 30, "a device", passing) is kept
