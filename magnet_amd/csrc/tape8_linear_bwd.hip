@@ -466,9 +466,9 @@ __global__ void __launch_bounds__(1024) k_tape8_linear_sum(const float* __restri
 }
 
 __global__ void __launch_bounds__(256) k_tape8_fill0(float* __restrict__ p, long ld, int rows, int cols) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < rows * cols) p[(i / cols) * ld + i % cols] = 0.f;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)rows * cols; i += (long)gridDim.x * 256) p[(i / cols) * ld + i % cols] = 0.f;
 }
+static unsigned t8_fill_grid(long n) { return (unsigned)(n < (1l << 28) ? (n + 255) / 256 : 1l << 20); }
 
 #define T8_BLOCK 128
 static int t8_pad(int n) { return n <= 64 ? 64 : 128; }                       // a block of at most 128 features, as 64 or 128
@@ -507,8 +507,8 @@ extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void
     hipStream_t st = (hipStream_t)stream;
     if (M == 0) {
         if (!accumulate) {
-            k_tape8_fill0<<<(N * K + 255) / 256, 256, 0, st>>>(dW, lddw, N, K);
-            if (db) k_tape8_fill0<<<(N + 255) / 256, 256, 0, st>>>(db, N, 1, N);
+            k_tape8_fill0<<<t8_fill_grid((long)N * K), 256, 0, st>>>(dW, lddw, N, K);
+            if (db) k_tape8_fill0<<<t8_fill_grid(N), 256, 0, st>>>(db, N, 1, N);
         }
         return (int)hipGetLastError();
     }

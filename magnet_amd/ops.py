@@ -911,6 +911,12 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
+def _apart(out, name, others):
+    for other, t in others:
+        if _overlap(out, t):
+            raise ValueError(f"magnet_amd: {name} must not overlap {other}")
+
+
 def tape8_pack(x, kind="signed", out=None) -> Tape8:
     """x [M, W] (fp32, bf16 or fp16) onto an 8-bit tape (csrc/tape8_kernels.hip)"""
     if kind not in TAPE8_KINDS:
@@ -918,6 +924,9 @@ def tape8_pack(x, kind="signed", out=None) -> Tape8:
     x = _matrix(x, "x", tuple(_T8_DTYPES))
     M, W = x.shape
     t = _tape8_ok(out, "out", kind, W, M) if out is not None else None
+    if t is not None:
+        _apart(t.codes, "out", [("x", x), ("itself", t.bytes)])
+        _apart(t.bytes, "out", [("x", x)])
     _on_device(x, t)
     if t is None:
         t = tape8_empty(M, W, kind, x.device)
@@ -931,9 +940,11 @@ def tape8_unpack(t: Tape8, dtype=torch.float32, out=None):
     _tape8_ok(t)
     if dtype not in _T8_DTYPES:
         raise TypeError(f"magnet_amd: a tape is read as {', '.join(str(d) for d in _T8_DTYPES)} (got {dtype})")
-    _on_device(t)
-    y = _out_matrix(out, "out", dtype, (t.rows, t.width), t.codes.device)
-    _on_device(y)
+    if out is not None:
+        _out_matrix(out, "out", dtype, (t.rows, t.width), None)
+        _apart(out, "out", [("the tape", t.codes), ("the tape", t.bytes)])
+    _on_device(t, out)
+    y = torch.empty(t.rows, t.width, dtype=dtype, device=t.codes.device) if out is None else out
     L.check(_entry("magnet_tape8_unpack", "pplii" "pil")(t.codes.data_ptr(), t.bytes.data_ptr(), t.rows, t.width, TAPE8_KINDS[t.kind], y.data_ptr(),
                                                          _T8_DTYPES[dtype], _ld(y), _raw_stream(_cur_dev())), "tape8_unpack")
     return y
@@ -971,11 +982,12 @@ def tape8_linear_bwd(dz, tape: Tape8, w, act="none", *, need_dx=True, dx=None, d
     _tape8_ok(tape, "tape", "relu" if act == "relu" else "signed", K, M)
     if accumulate and (dW is None or db is None):
         raise ValueError("magnet_amd: accumulate needs the dW and db to add to")
+    taken = [("dz", dz), ("w", w), ("the tape", tape.codes), ("the tape", tape.bytes)]
     for o, name, shape in ((dx, "dx", (M, K)), (dW, "dW", (N, K)), (db, "db", (N,))):
-        if o is not None and _overlap(_out_matrix(o, name, torch.float32, shape, None), dz):
-            raise ValueError(f"magnet_amd: {name} must not overlap dz")
-        if o is not None and _overlap(o, w):
-            raise ValueError(f"magnet_amd: {name} must not overlap w")
+        if o is not None:
+            _out_matrix(o, name, torch.float32, shape, None)
+            _apart(o, name, taken)
+            taken.append((name, o))
     _on_device(dz, tape, w, dx, dW, db)
     dev = dz.device
     if need_dx and dx is None:
@@ -1094,6 +1106,7 @@ def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_
     """The backward pass of ``norm_join`` from the gradients of y and h (with a pre norm) and what its ``tape`` kept; post, pre, gate, scale and
     norm as handed to it.  Gradients of x, f and gate have gy's type, those of parameters are fp32.  ``need_x`` False: no gradient of x
     (without a pre norm it is gy)."""
+    one_gate = isinstance(gate, torch.Tensor) and gate.dim() == 1
     gy, (pg, pb), (qg, qb), gate, G, sv, sc = _join_args(gy, "gy", post, pre, gate, scale, norm)
     M, W = gy.shape
     if (gh is None) != (qg is None):
@@ -1113,7 +1126,7 @@ def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_
     fill = torch.empty if M else torch.zeros                # (no rows: no launch)
     new = lambda *s: fill(*s, dtype=gy.dtype, device=dev)  # noqa: E731
     par = lambda p: fill(W, dtype=torch.float32, device=dev) if p is not None else None  # noqa: E731
-    g = NormJoinGrads(new(M, W) if need_x else None, new(M, W), new(*gate.shape) if gate is not None else None, par(sv),
+    g = NormJoinGrads(new(M, W) if need_x else None, new(M, W), new(*((W,) if one_gate else gate.shape)) if gate is not None else None, par(sv),
                       (par(pg), par(pb)) if pg is not None else None, (par(qg), par(qb)) if qg is not None else None)
     if M == 0:
         return g

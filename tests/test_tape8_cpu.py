@@ -174,3 +174,27 @@ def test_a_tape_is_kept_only_where_the_rows_that_become_it_fit(monkeypatch):
     for passing, kept in ((0, True), (40 << 30, True), (60 << 30, False)):
         monkeypatch.setattr(AG, "_MEM", dict(dev=None, t=0.0, total=0, free=0, granted=0))
         assert AG._keep_tape(15 << 30, "a device", passing) is kept
+
+
+def test_outputs_share_no_memory():
+    """an output on top of an input, of the tape or of another output is refused (the rows are walked in no order)"""
+    dz, w = torch.randn(6, 8), torch.randn(8, 40)
+    both = torch.empty(400)
+    for kw, names in ((dict(dW=both[:320].view(8, 40), db=both[319:327]), "db must not overlap dW"),
+                      (dict(dx=both[:240].view(6, 40), dW=both[80:].view(8, 40)), "dW must not overlap dx")):
+        with pytest.raises(ValueError, match=names):
+            ops.tape8_linear_bwd(dz, tape(6, 40), w, **kw)
+    mem = torch.zeros(6, 40)
+    t = ops.Tape8(mem.view(torch.uint8).view(-1)[:6 * 64].view(6, 64), torch.zeros(6, 2, dtype=torch.uint8), 40)
+    with pytest.raises(ValueError, match="dx must not overlap the tape"):
+        ops.tape8_linear_bwd(dz, t, w, dx=mem)
+    with pytest.raises(ValueError, match="out must not overlap x"):
+        ops.tape8_pack(mem, out=t)
+    with pytest.raises(ValueError, match="out must not overlap the tape"):
+        ops.tape8_unpack(t, out=mem)
+    t.codes, t.bytes = torch.zeros(6, 64, dtype=torch.uint8), mem.view(torch.uint8).view(-1)[100:112].view(6, 2)
+    with pytest.raises(ValueError, match="out must not overlap x"):
+        ops.tape8_pack(mem, out=t)
+    t.bytes = t.codes.view(-1)[12:24].view(6, 2)
+    with pytest.raises(ValueError, match="out must not overlap itself"):
+        ops.tape8_pack(mem, out=t)

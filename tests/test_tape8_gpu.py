@@ -257,6 +257,16 @@ def test_linear_bwd_outputs_strides_and_accumulate():
     assert bool((a == 2.0).all()) and bool((b == 3.0).all())
 
 
+def test_linear_bwd_no_rows_of_a_large_weight():
+    """more than 2^31 values of dW to clear"""
+    from magnet_amd import ops
+    n = 46400
+    w = torch.empty(n, n, device="cuda")
+    dW = torch.ones(n, n, device="cuda")
+    _, a, b = ops.tape8_linear_bwd(torch.empty(0, n, device="cuda"), ops.tape8_empty(0, n), w, dW=dW)
+    assert a is dW and not any(bool(rows.any()) for rows in dW.split(4096)) and not b.any()
+
+
 def test_linear_bwd_one_buffer_for_several_gradients():
     """dW and db inside wider buffers, N in two blocks of 128: neighbours are left alone"""
     from magnet_amd import ops
@@ -472,6 +482,18 @@ def test_norm_join_strides():
         assert torch.equal(r.y, want.y) and torch.equal(r.h, want.h) and torch.equal(r.post_tape.codes, want.post_tape.codes)
     one = ops.norm_join(**{**c, "gate": c["gate"][0]})
     assert torch.equal(one.y, ops.norm_join(**{**c, "gate": c["gate"][:1].expand(50, 100).contiguous()}).y)
+
+
+@pytest.mark.parametrize("M", [0, 50])
+def test_norm_join_one_gate_for_all_rows(M):
+    """a gate of shape [W] gets a gradient of that shape, the one that [1, W] gets"""
+    from magnet_amd import ops
+    c = join_case(M, 100, 1, "rms", True, False, False, torch.float32)
+    r = ops.norm_join(**c, tape=True)
+    args = dict(post_tape=r.post_tape, post_rstd=r.post_rstd, post=c["post"], scale=c["scale"], norm="rms")
+    gy = torch.randn(M, 100, device="cuda")
+    a, b = (ops.norm_join_bwd(gy, gate=g, **args) for g in (c["gate"], c["gate"][0]))
+    assert a.gate.shape == (1, 100) and b.gate.shape == (100,) and torch.equal(a.gate[0], b.gate) and torch.equal(a.f, b.f)
 
 
 def test_norm_join_no_rows():
