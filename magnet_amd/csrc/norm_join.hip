@@ -36,6 +36,7 @@ struct NjArgs {
     long rows_per_gate;                  // M / G (M without a gate)
     long groups;                         // backward: G, 1 without a gate
     int W, layer, has_post, has_pre, has_gate, tape, per_group, need_sums;
+    int plain_sums;                      // backward: S0 and P0 too (somebody has a bias)
     float scale, eps;
 };
 
@@ -72,8 +73,8 @@ __device__ __forceinline__ void nj_sum(float& a, float& b, NjRed& red, int& turn
     if (TL > 64) {
         constexpr int NW = TL / 64;
         if (!(threadIdx.x & 63)) {
-            red.v[turn][0][threadIdx.x >> 6] = a;
-            if (BOTH) red.v[turn][1][threadIdx.x >> 6] = b;
+            red.v[turn][0][threadIdx.x % TL >> 6] = a;
+            if (BOTH) red.v[turn][1][threadIdx.x % TL >> 6] = b;
         }
         wg_barrier();
         a = 0.f;
@@ -237,11 +238,12 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join(const NjArgs 
 //   G gate rows, few: per_group workgroups for each, their sums stay apart (S1, S0 without the gate) and meet in k_norm_join_gate
 //   many (OWN):       a team takes whole gate rows one after the other - up to one for every row - and writes their gradients itself
 template <typename T, int TL, int VPT, bool OWN>
-__global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjArgs a) {
-    __shared__ NjRed red;
-    constexpr int NT = TL > 256 ? TL : 256, TEAMS = NT / TL;
+__global__ void __launch_bounds__(TL > 64 ? 512 : 256) k_norm_join_bwd(const NjArgs a) {
+    constexpr int NT = TL > 64 ? 512 : 256, TEAMS = NT / TL;
+    __shared__ NjRed reds[TL > 64 ? TEAMS : 1];
     __shared__ __attribute__((aligned(16))) float part[TEAMS > 1 ? NT * 4 : 4];
     const int lane = threadIdx.x % TL, team = threadIdx.x / TL, W = a.W, blocks = (W + 31) / 32;
+    NjRed& red = reds[TL > 64 ? team : 0];
     const T *gy = (const T*)a.x, *gh = (const T*)a.f, *gate = (const T*)a.gate;
     T *dx = (T*)a.y, *df = (T*)a.h, *dgate = (T*)a.dgate;
     int turn = 0;
@@ -258,8 +260,11 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
     long g = OWN ? me : a.per_group ? blockIdx.x / a.per_group : 0;
     const long step = OWN ? 1 : (long)(a.per_group ? a.per_group : gridDim.x) * TEAMS;
     long row = g * a.rows_per_gate + (OWN ? 0 : a.per_group ? (long)(blockIdx.x % a.per_group) * TEAMS + team : me);
-    long last = min(g + 1, a.groups) * a.rows_per_gate;
-    bool more = g < a.groups && row < last;
+    long last = (g + 1) * a.rows_per_gate;
+    // teams of several waves meet at the workgroup's barriers: all of them go round as often as the first one, which has the most rows (OWN: rows
+    // and last move alike in all teams, past the last gate row too)
+    const int lead = TL > 64 ? team : 0;
+    bool more = OWN ? g - lead < a.groups : row - lead < last, on = OWN ? g < a.groups : row < last;
     nj_raw<T> ny[VPT], nh[VPT], ng[VPT];
     unsigned npc[VPT], nqc[VPT], npe[VPT], nqe[VPT];
     float npr = 1.f, nqr = 1.f;
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
     t8_f4 S1[VPT], S0[VPT], P1[VPT], P0[VPT], T1[VPT], T0[VPT];               // T: of the gate row so far, without the gate
 #pragma unroll
     for (int i = 0; i < VPT; ++i) S1[i] = S0[i] = P1[i] = P0[i] = T1[i] = T0[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
-    if (more) load(row, g);
+    if (on) load(row, g);
     while (more) {
         t8_f4 D[VPT], v[VPT], gt[VPT], u[VPT], q[VPT];
 #pragma unroll
@@ -299,23 +304,24 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
         const float pr = npr, qr = nqr;
         // the row after this one, on its way while this one is worked on
         const long r = row, gr = g;
+        const bool here = TL > 64 ? __builtin_amdgcn_readfirstlane(on) : true;
         row += step;
         bool ends = false;
-        if (row >= last) {
-            ends = true;
-            if (OWN) {
+        if (OWN) {
+            ends = row >= last;
+            if (ends) {
                 g += g_step;
                 row = g * a.rows_per_gate, last = row + a.rows_per_gate;
-                more = g < a.groups;
-            } else {
-                more = false;
+                more = g - lead < a.groups, on = g < a.groups;
             }
+        } else {
+            more = row - lead < last, on = row < last;
         }
-        if (more) load(row, g);
+        if (on) load(row, g);
         if (a.has_pre) {
 #pragma unroll
             for (int i = 0; i < VPT; ++i) {
-                P0[i] += u[i], P1[i] += u[i] * q[i];
+                if (here) P0[i] += u[i], P1[i] += u[i] * q[i];
                 u[i] *= qg[i];
             }
             nj_norm_bwd<TL, VPT>(u, q, qr, lane, a, red, turn);
@@ -325,14 +331,17 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
-            if (dx) t8_store4(dx + r * a.ldy + c, W - c, D[i]);
-            T0[i] += D[i], T1[i] += D[i] * v[i];
+            if (here) {
+                if (dx) t8_store4(dx + r * a.ldy + c, W - c, D[i]);
+                T0[i] += D[i], T1[i] += D[i] * v[i];
+            }
             D[i] *= gt[i] * sc[i] * pg[i];
         }
         if (a.has_post) nj_norm_bwd<TL, VPT>(D, v, pr, lane, a, red, turn);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = 4 * (i * TL + lane);
+            if (!here) break;
             t8_store4(df + r * a.ldh + c, W - c, D[i]);
             if (OWN && ends) {
                 t8_store4(dgate + gr * W + c, W - c, (T1[i] * pg[i] + T0[i] * pb[i]) * sc[i]);
@@ -345,7 +354,8 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
     // ---- the workgroup's sums: the teams in order
     float* out = a.part + (size_t)blockIdx.x * 4 * W;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < 4; ++q) {
+        if ((q & 1) && !a.plain_sums) continue;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             t8_f4 s = q == 0 ? (OWN ? S1[i] : T1[i]) : q == 1 ? (OWN ? S0[i] : T0[i]) : q == 2 ? P1[i] : P0[i];
@@ -364,10 +374,12 @@ __global__ void __launch_bounds__(TL > 256 ? TL : 256) k_norm_join_bwd(const NjA
                 for (int k = 0; k < 4; ++k)
                     if (c + k < W) out[q * W + c + k] = s[k];
         }
+    }
 }
 
 // sums of a column over n of the workgroups' sets (`first`, first + apart, ..), in order: a workgroup takes 32 columns, 32 slices of the sets each; the total in
-// v of slice 0
+// v of slice 0.  STEP 2: of S1 and P1 alone
+template <int STEP>
 __device__ __forceinline__ void nj_fold(const float* part, long first, int n, long apart, int W, int c, float (&v)[4], float (*s)[4][32]) {
     const int col = threadIdx.x & 31, slice = threadIdx.x >> 5;
 #pragma unroll
@@ -377,26 +389,26 @@ __device__ __forceinline__ void nj_fold(const float* part, long first, int n, lo
         for (int w = slice; w < n; w += 32) {
             const float* p = part + (first + w * apart) * 4 * W + c;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] += p[(long)q * W];
+            for (int q = 0; q < 4; q += STEP) v[q] += p[(long)q * W];
         }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) s[slice][q][col] = v[q];
+    for (int q = 0; q < 4; q += STEP) s[slice][q][col] = v[q];
     __syncthreads();
     if (slice) return;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 4; q += STEP) {
         v[q] = s[0][q][col];
         for (int k = 1; k < 32; ++k) v[q] += s[k][q][col];
     }
 }
 // one gate row (blockIdx.y): its gradient, and its workgroups' sums with the gate multiplied in, left in the first one's place
-template <typename T>
+template <typename T, int STEP>
 __global__ void __launch_bounds__(1024) k_norm_join_gate(const NjArgs a) {
     __shared__ float s[32][4][32];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), W = a.W;
     const long g = blockIdx.y;
     float v[4];
-    nj_fold(a.part, g * a.per_group, a.per_group, 1, W, c, v, s);
+    nj_fold<STEP>(a.part, g * a.per_group, a.per_group, 1, W, c, v, s);
     if (threadIdx.x >= 32 || c >= W) return;
     const float gt = (float)((const T*)a.gate)[g * a.ldg + c], sc = a.scale_v ? a.scale_v[c] : a.scale;
     const float t = v[0] * (a.has_post ? a.post_g[c] : 1.f) + (a.post_b ? v[1] * a.post_b[c] : 0.f);
@@ -405,12 +417,13 @@ __global__ void __launch_bounds__(1024) k_norm_join_gate(const NjArgs a) {
     p[0] = gt * v[0], p[W] = gt * v[1], p[2 * W] = v[2], p[3 * W] = v[3];
 }
 // the parameters' gradients from n sets of sums, `apart` sets from one to the next
+template <int STEP>
 __global__ void __launch_bounds__(1024) k_norm_join_params(const NjArgs a, int n, int apart, float* d_scale, float* d_post_g, float* d_post_b, float* d_pre_g,
                                                           float* d_pre_b) {
     __shared__ float s[32][4][32];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31);
     float v[4];
-    nj_fold(a.part, 0, n, apart, a.W, c, v, s);
+    nj_fold<STEP>(a.part, 0, n, apart, a.W, c, v, s);
     if (threadIdx.x >= 32 || c >= a.W) return;
     const float sc = a.scale_v ? a.scale_v[c] : a.scale;
     if (d_scale) d_scale[c] = v[0] * (a.has_post ? a.post_g[c] : 1.f) + (a.post_b ? v[1] * a.post_b[c] : 0.f);
@@ -429,21 +442,23 @@ __global__ void __launch_bounds__(1024) k_norm_join_params(const NjArgs a, int n
 // so that a workgroup of four waves is one row's)
 static int nj_team(int W) { return W <= 128 ? 16 : W <= 256 ? 32 : W <= 512 ? 64 : W <= 2048 ? 256 : 512; }
 static int nj_teams(int W) { return W <= 2048 ? 256 / nj_team(W) : 1; }
+// one row a team while that makes at most 1024 workgroups, then four rows a team (the parameters are loaded once for all of them): 262 144 x 128
+// with tapes 166 us (one row a team 180, sixteen 174), 8190 x 2048 39 us (50, 44); at most 4096 workgroups
 static long nj_grid(long M, int W) {
     const int teams = nj_teams(W);
     const long n = (M + teams - 1) / teams;
-    return n < 1024 ? n : 1024;
+    return n < 1024 ? n : n < 4096 ? 1024 : n < 16384 ? n / 4 : 4096;
 }
 // backward: workgroups, and how many of them share a gate row (0: they are not bound to gate rows).  Up to 2048 gate rows get workgroups of
 // their own - a set of sums each, added by a second launch; beyond that a team walks whole gate rows and no sums are kept per row
 static long nj_bwd_grid(long M, int W, long G, int* per_group) {
-    const int teams = nj_teams(W);
+    const int teams = W <= 512 ? nj_teams(W) : 512 / nj_team(W), most = W <= 1024 ? NJ_MOST : 256;
     *per_group = 0;
     if (G <= 0 || G > 2048 || G == M) {
         const long n = ((G > 2048 ? G : M) + teams - 1) / teams;
-        return n < NJ_MOST ? n : NJ_MOST;
+        return n < most ? n : most;
     }
-    const long each = (M / G + teams - 1) / teams, n = G < 512 ? 512 / G : 1;
+    const long each = (M / G + teams - 1) / teams, n = G < most ? most / G : 1;
     *per_group = (int)(each < n ? each : n);
     return G * *per_group;
 }
@@ -473,8 +488,8 @@ static void nj_backward(const NjArgs& a, dim3 grid, hipStream_t st) {
     else if (W <= 128) k_norm_join_bwd<T, 16, 2, OWN><<<grid, 256, 0, st>>>(a);
     else if (W <= 256) k_norm_join_bwd<T, 32, 2, OWN><<<grid, 256, 0, st>>>(a);
     else if (W <= 512) k_norm_join_bwd<T, 64, 2, OWN><<<grid, 256, 0, st>>>(a);
-    else if (W <= 1024) k_norm_join_bwd<T, 256, 1, OWN><<<grid, 256, 0, st>>>(a);
-    else if (W <= 2048) k_norm_join_bwd<T, 256, 2, OWN><<<grid, 256, 0, st>>>(a);
+    else if (W <= 1024) k_norm_join_bwd<T, 256, 1, OWN><<<grid, 512, 0, st>>>(a);
+    else if (W <= 2048) k_norm_join_bwd<T, 256, 2, OWN><<<grid, 512, 0, st>>>(a);
     else k_norm_join_bwd<T, 512, 2, OWN><<<grid, 512, 0, st>>>(a);
 }
 extern "C" int magnet_norm_join(const void* x, long ldx, const void* f, long ldf, int dtype, long M, int W, int layer, float eps, const float* post_g,
@@ -526,16 +541,17 @@ extern "C" int magnet_norm_join_bwd(const void* gy, long ldgy, const void* gh, l
     const long grid = nj_bwd_grid(M, W, gate ? G : 0, &a.per_group);
     a.groups = gate ? G : 1;
     a.need_sums = a.per_group || d_scale || d_post_g || d_post_b || d_pre_g || d_pre_b;
+    a.plain_sums = post_b || d_post_b || d_pre_b;
     hipStream_t st = (hipStream_t)stream;
     const bool own = gate && !a.per_group;
     if (dtype == T8_F32) own ? nj_backward<float, true>(a, dim3((unsigned)grid), st) : nj_backward<float, false>(a, dim3((unsigned)grid), st);
     else own ? nj_backward<__bf16, true>(a, dim3((unsigned)grid), st) : nj_backward<__bf16, false>(a, dim3((unsigned)grid), st);
     const dim3 pg((W + 31) / 32, a.per_group ? (unsigned)G : 1);
     if (a.per_group) {
-        if (dtype == T8_F32) k_norm_join_gate<float><<<pg, 1024, 0, st>>>(a);
-        else k_norm_join_gate<__bf16><<<pg, 1024, 0, st>>>(a);
+        if (dtype == T8_F32) a.plain_sums ? k_norm_join_gate<float, 1><<<pg, 1024, 0, st>>>(a) : k_norm_join_gate<float, 2><<<pg, 1024, 0, st>>>(a);
+        else a.plain_sums ? k_norm_join_gate<__bf16, 1><<<pg, 1024, 0, st>>>(a) : k_norm_join_gate<__bf16, 2><<<pg, 1024, 0, st>>>(a);
     }
     if (d_scale || d_post_g || d_post_b || d_pre_g || d_pre_b)
-        k_norm_join_params<<<dim3(pg.x), 1024, 0, st>>>(a, a.per_group ? (int)G : (int)grid, a.per_group ? a.per_group : 1, d_scale, d_post_g, d_post_b, d_pre_g, d_pre_b);
+        (a.plain_sums ? k_norm_join_params<1> : k_norm_join_params<2>)<<<dim3(pg.x), 1024, 0, st>>>(a, a.per_group ? (int)G : (int)grid, a.per_group ? a.per_group : 1, d_scale, d_post_g, d_post_b, d_pre_g, d_pre_b);
     return (int)hipGetLastError();
 }

@@ -469,6 +469,16 @@ def test_norm_join_backward(dtype, norm, M, W, G):
         assert all(torch.equal(a, b) for k in ("post", "pre") for a, b in zip(getattr(g, k) or (), getattr(again, k) or ()) if a is not None)
 
 
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("M,W,G", [(4099, 600, 4099), (4098, 700, 2049), (2051, 1000, 0), (1027, 1500, 1027), (4202, 1100, 2101), (603, 2000, 3), (1, 1000, 1),
+                                   (515, 2500, 515), (65537, 20, 0)])
+def test_norm_join_workgroups_of_several_rows(norm, M, W, G):
+    """wide rows two at a time in a workgroup, the last one alone; gate rows one and two at a time"""
+    for dtype in ("fp32", "bf16"):
+        test_norm_join_forward(dtype, norm, M, W, G)
+        test_norm_join_backward(dtype, norm, M, W, G)
+
+
 def test_norm_join_strides():
     """rows inside wider arrays, aligned to 16 bytes and not, give the same bits"""
     from magnet_amd import ops
