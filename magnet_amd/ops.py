@@ -836,16 +836,18 @@ def _tape8_ok(t: Tape8, name="tape", kind=None, width=None, rows=None) -> Tape8:
     nb = (t.width + 31) // 32
     if t.kind not in TAPE8_KINDS or t.width < 1:
         raise ValueError(f"magnet_amd: {name}: kind {t.kind!r}, width {t.width}")
-    for a, w in ((t.codes, 32 * nb), (t.bytes, nb)):
-        _is_tensor(a, name)
-        if a.dtype != torch.uint8 or a.dim() != 2 or a.shape[1] != w or a.shape[0] != t.codes.shape[0] or not a.is_contiguous():
-            raise ValueError(f"magnet_amd: {name}: a tape of width {t.width} is contiguous uint8 codes [M, {32 * nb}] and bytes [M, {nb}] "
-                             f"(got {tuple(t.codes.shape)} and {tuple(t.bytes.shape)})")
-    if t.codes.data_ptr() & 15:
+    c, b = t.codes, t.bytes
+    _is_tensor(c, name)
+    _is_tensor(b, name)
+    M = c.shape[0] if c.dim() else 0
+    if c.shape != (M, 32 * nb) or b.shape != (M, nb) or c.dtype != torch.uint8 or b.dtype != torch.uint8 or not c.is_contiguous() or not b.is_contiguous():
+        raise ValueError(f"magnet_amd: {name}: a tape of width {t.width} is contiguous uint8 codes [M, {32 * nb}] and bytes [M, {nb}] "
+                         f"(got {tuple(c.shape)} and {tuple(b.shape)})")
+    if c.data_ptr() & 15:
         raise ValueError(f"magnet_amd: {name}: the codes must be 16-byte aligned")
     if kind is not None and t.kind != kind:
         raise ValueError(f"magnet_amd: {name} is a {t.kind!r} tape, a {kind!r} one is needed")
-    if (width is not None and t.width != width) or (rows is not None and t.rows != rows):
+    if (width is not None and t.width != width) or (rows is not None and M != rows):
         raise ValueError(f"magnet_amd: {name} has {t.rows} rows of width {t.width}, expected {rows} of {width}")
     return t
 
@@ -857,17 +859,17 @@ def _is_tensor(t, name):
 
 def _on_device(*tensors):
     """every tensor that is there lives on the current HIP device (checked last: a call that is wrong anyway says so on any machine)"""
-    cur = -1
+    cur = -2                                                              # (not asked yet; a CPU tensor's is -1)
     for t in tensors:
-        for u in ((t.codes, t.bytes) if isinstance(t, Tape8) else (t,)):
-            if u is None:
-                continue
-            if not u.is_cuda:
-                raise RuntimeError(f"magnet_amd: a tensor must live on a HIP device (got {u.device}); there is no CPU path")
-            if cur < 0:
-                cur = _cur_dev()
+        if t is None:
+            continue
+        for u in (t.codes, t.bytes) if type(t) is Tape8 else (t,):
             if u.get_device() != cur:
-                _same_device(u, "a tensor")
+                if not u.is_cuda:
+                    raise RuntimeError(f"magnet_amd: a tensor must live on a HIP device (got {u.device}); there is no CPU path")
+                cur = _cur_dev()
+                if u.get_device() != cur:
+                    _same_device(u, "a tensor")
 
 
 def _matrix(t, name, dtypes, shape=None):
@@ -1125,7 +1127,9 @@ def norm_join_bwd(gy, gh=None, *, post_tape, post_rstd=None, pre_tape=None, pre_
     dev = gy.device
     fill = torch.empty if M else torch.zeros                # (no rows: no launch)
     new = lambda *s: fill(*s, dtype=gy.dtype, device=dev)  # noqa: E731
-    par = lambda p: fill(W, dtype=torch.float32, device=dev) if p is not None else None  # noqa: E731
+    some = [p is not None for p in (sv, pg, pb, qg, qb)]
+    vectors = iter(fill(sum(some), W, dtype=torch.float32, device=dev).unbind(0) if any(some) else ())      # (one allocation for all)
+    par = lambda p: next(vectors) if p is not None else None  # noqa: E731
     g = NormJoinGrads(new(M, W) if need_x else None, new(M, W), new(*((W,) if one_gate else gate.shape)) if gate is not None else None, par(sv),
                       (par(pg), par(pb)) if pg is not None else None, (par(qg), par(qb)) if qg is not None else None)
     if M == 0:
