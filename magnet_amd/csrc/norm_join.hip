@@ -14,7 +14,7 @@
 // All four sums over rows are linear in  S1 = sum gate D f^,  S0 = sum gate D,  P1 = sum gh y^,  P0 = sum gh  - four sums per column.
 //
 // Both are bound by HBM: every array is read or written once.  Measured at 262 144 x 128 fp32 with a gate for each of four runs of rows:
-// with both tapes 128 us (4.7 TB/s), backward 117 + 9 us for the parameters' sums (4.7 TB/s); a large copy reaches 4.9.  A row belongs to a team of 16 to 512 lanes, four neighbouring columns per
+// with both tapes 122 us (5.0 TB/s), backward 117 + 9 us for the parameters' sums (4.7 TB/s); a large copy reaches 4.9.  A row belongs to a team of 16 to 512 lanes, four neighbouring columns per
 // lane and slot, at most two slots: it stays in registers from its load to its last use, and the next row of the team is loaded before this
 // one is worked on (the statistics are two dependent sums over the row: without rows in flight behind them the loads' latency is what
 // the kernel takes).  Sums over a team are lane exchanges inside the vector unit, through LDS for a team of several waves; fp32, the
@@ -435,9 +435,6 @@ __global__ void __launch_bounds__(1024) k_norm_join_params(const NjArgs a, int n
 
 // ---------------------------------------------------------------------------------------------------------------------------- launches
 #define NJ_MAX_W 4096
-#ifndef NJ_MOST
-#define NJ_MOST 512
-#endif
 // lanes of a row's team: two slots of four columns each, sixteen lanes at least (rows of 513 .. 1024 values: four waves with one slot each,
 // so that a workgroup of four waves is one row's)
 static int nj_team(int W) { return W <= 128 ? 16 : W <= 256 ? 32 : W <= 512 ? 64 : W <= 2048 ? 256 : 512; }
@@ -450,9 +447,12 @@ static long nj_grid(long M, int W) {
     return n < 1024 ? n : n < 4096 ? 1024 : n < 16384 ? n / 4 : 4096;
 }
 // backward: workgroups, and how many of them share a gate row (0: they are not bound to gate rows).  Up to 2048 gate rows get workgroups of
-// their own - a set of sums each, added by a second launch; beyond that a team walks whole gate rows and no sums are kept per row
+// their own - a set of sums each, added by a second launch; beyond that a team walks whole gate rows and no sums are kept per row.  Rows of
+// 513 .. 2048 values go two at a time in a workgroup of eight waves: twice the rows in flight for the same partial sums (20 000 x 1000: 88 us, one at a
+// time 102; bf16 61, 80).  What the registers hold of a CU's rows is 512 workgroups up to a width of 1024, 256 beyond (bf16 8000 x 2048: 64 us, 512
+// of them 72; 8000 rows of 4096: 146, 155)
 static long nj_bwd_grid(long M, int W, long G, int* per_group) {
-    const int teams = W <= 512 ? nj_teams(W) : 512 / nj_team(W), most = W <= 1024 ? NJ_MOST : 256;
+    const int teams = W <= 512 ? nj_teams(W) : 512 / nj_team(W), most = W <= 1024 ? 512 : 256;
     *per_group = 0;
     if (G <= 0 || G > 2048 || G == M) {
         const long n = ((G > 2048 ? G : M) + teams - 1) / teams;
