@@ -15,12 +15,17 @@
 // The error of both is a few 2^-22 of the operands' magnitude, sums are held in fp32, and the workgroups' partial sums of dW and db are added
 // in their order by a second kernel: the same bits every time.
 //
-// Scales.  fp16 spans 2^40; gradients (1e-7) and tapes (any byte) do not fit by themselves.  The workgroup keeps a bound on the exponents it has
-// met, of dz and of the tape's bytes, and stages everything times the power of two that puts the bound near the top of the range.  A lane
-// that meets more raises a flag with its write; behind the barrier that the step has anyway all waves see it, add their sums so far to the
-// workgroup's partial sums in memory and begin again under a new bound (with a few binades to spare): rare after the first step, and
-// nobody waits for a maximum otherwise.  (Scaling the sums in registers instead costs a second set of them: measured as spills.)  Rows
-// 2^-24 below the largest so far start to lose bits, of a share that small of the sums.  A wave scales its part of W likewise.
+// Scales.  fp16 spans 2^40; gradients (1e-7) and tapes (any byte) do not fit by themselves.  Every row of dz is staged times the power of two
+// that puts its own largest value into [2^14, 2^15), and dx undoes it row by row: a row of dx is as good as its row of dz, whatever the
+// others are, down to 2^-39 of the row's largest value.  dW needs all rows at one scale, so a row's codes take the difference: they are
+// staged times 2^(row's exponent + block's byte - bound + 5), one bound for each 32 columns of x: where the largest product of a row
+// of dz and a block lies, smaller ones lose what is under 2^-32 of it.  (Behind Swish the exponent of the value itself stands for the byte: far
+// from zero on the negative side it has nothing to do with the argument's.)  A lane that meets a product above its bound raises a flag
+// with its write; behind the barrier that the step has anyway all waves see it, add their sums so far to the workgroup's partial sums in
+// memory and begin again under a new bound (with a few binades to spare): rare after the first step, and nobody waits for a maximum
+// otherwise.  (Scaling the sums in registers instead costs a second set of them: measured as spills.)  A row's largest value is a few lane
+// permutes, and the wave that stages a row of dz stages its codes too, so the exponent never waits for another wave.  A wave scales its part
+// of W likewise, by the part's largest value.
 #include "common.cuh"
 #include "split_single.cuh"
 #include "tape8.cuh"
@@ -41,6 +46,29 @@ struct T8LinArgs {
     int N, K, ldc, exact, add_dx;        // exact: N = NP and K a multiple of KP; add_dx: dx += (a later block of N)
 };
 
+template <int CTRL>
+__device__ __forceinline__ unsigned t8_dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
+// the maxima of P values each over L = 16 or 32 neighbouring lanes: value p's comes out in the lanes whose number is p modulo P
+template <int P, int L>
+__device__ __forceinline__ unsigned t8_row_max(const unsigned (&m)[P], int lane) {
+    static_assert(P == 2 || P == 4, "two or four values");
+    const bool odd = lane & 1, two = lane & 2;
+    unsigned v = max(odd ? m[1] : m[0], t8_dpp<0xB1>(odd ? m[0] : m[1]));                       // quad_perm 1 0 3 2: the neighbour hands over what it is not for
+    if (P == 4) {
+        const unsigned w = max(odd ? m[P - 1] : m[P - 2], t8_dpp<0xB1>(odd ? m[P - 2] : m[P - 1]));
+        v = max(two ? w : v, t8_dpp<0x4E>(two ? v : w));                                      // quad_perm 2 3 0 1
+    } else {
+        v = max(v, t8_dpp<0x4E>(v));
+    }
+    v = max(v, t8_dpp<0x124>(v));                                                             // row_ror 4, 8: the other quads of sixteen lanes
+    v = max(v, t8_dpp<0x128>(v));
+    if (L == 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        const unsigned r0 = r[0], r1 = r[1];
+        v = max(r0, r1);
+    }
+    return v;
+}
 // exponent byte (1 .. 254) of a magnitude's bits; 0 for zero, subnormals and what is not finite
 __device__ __forceinline__ unsigned t8_expo(float v) {
     const unsigned e = (__float_as_uint(v) >> 23) & 0xFFu;
@@ -72,14 +100,16 @@ __device__ __forceinline__ float t8_swish(float v, float& d) {
 #define T8_TILE(NP, KP, ACT) ((NP) == 128 && (KP) == 128 && (ACT) == ACT_SWISH ? 1 : 2)       // blocks of 16 features of a wave's tiles
 #define T8_FOLD 8                        // steps whose products are added up in a row before they join the sums so far: a chain of additions in fp32
                                          // is off by its length (2 097 152 rows: 1.7e-6 of dW in one chain per workgroup)
-#define T8_ZROOM 3                       // binades of dz and of the tape's bytes that may still come before the scale has to change
-#define T8_XROOM 2
+// binades by which the products of dz and x may still grow before the scale has to change (behind Swish, whose values spread wider than a tape's
+// bytes, and have a bit more of fp16's range, one more)
+#define T8_ROOM(ACT) ((ACT) == ACT_SWISH ? 4 : 3)
 template <int NP, int KP, int XPL, int R, int ACT>
 struct T8Step {                          // a step of R rows in LDS; row strides of 16 halfwords more than a power of two spread the rows over the banks
     unsigned short z[2][R][NP + 16];
     unsigned short x[XPL][R][KP + 16];
     unsigned c[ACT == ACT_RELU ? R : 1][KP / 4 + 4];       // the codes (the mask of dx)
     float d[ACT == ACT_SWISH ? R : 1][KP + 4];             // Swish's derivative: formed where Swish is, from the same exponential
+    int e[R];                                              // the rows' exponents: z is dz times 2^(141 - e)
 };
 
 // a value at a wave-uniform base plus the lane's offset in bytes (global_* with a scalar base: the caller hides the base behind an asm statement,
@@ -108,23 +138,26 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     constexpr int R = T8_ROWS(NP, KP, ACT);
     typedef T8Step<NP, KP, XPL, R, ACT> Step;
     constexpr int NW = T8_WAVES(NP, KP), LANES = 64 * NW;
-    constexpr int LPR = NP / 4, RPL = LANES / LPR, NLD = R / RPL;             // lanes per row of dz, rows per pass, passes
+    // a wave stages WR neighbouring rows, of dz and of the codes
+    constexpr int LPR = NP / 4, WR = R / NW, NLD = WR * LPR / 64;             // lanes per row of dz, rows (one after the other) of each such lane
     constexpr int CPT = R * KP / LANES, CPR = KP / CPT, CW = CPT / 4;        // codes per lane (8 or 16), lanes per row, words
+    static_assert(WR * CPR == 64 && LPR == NLD * CPR, "LPR neighbouring lanes hold the codes of their rows of dz");
     // a wave's part: dx of NBK blocks of 16 features and 1 / RW of the rows; dW of NBN blocks of features of dz and KB of features of x
     constexpr int NBK = T8_TILE(NP, KP, ACT), NBN = NBK, NT = NP / 32;
     constexpr int KW = KP / 16 / NBK, RW = NW / KW, RBS = R / 16 / RW, RB = RBS < 2 ? RBS : 2;
     constexpr int NG = NP / 16 / NBN, XG = NW / NG, KB = KP / 16 / XG;
+    constexpr int TB = KB / 2, CB = KP / 32, LB = 32 / CPT;                   // blocks of 32 columns: of the wave's dW, of all; lanes per block
     static_assert(KW * RW == NW && NG * XG == NW && RBS * 16 * RW == R, "waves tile both products");
     typedef unsigned t8_cw __attribute__((ext_vector_type(CW)));
     __shared__ __attribute__((aligned(16))) Step sb[2];
-    __shared__ unsigned red[NW], flag[2];
+    __shared__ unsigned red[NW][CB], flag[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
     const int k0 = blockIdx.y * KP;
     const int kf = 16 * NBK * (wave % KW), wr = (wave / KW) * (R / RW);       // its features and rows of dx
     const int nf = 16 * NBN * (wave % NG), xf = 16 * KB * (wave / NG);        // its features of dz and of x in dW
     // ---- what this lane loads of a step
-    const int zr = tid / LPR, zc = 4 * (tid % LPR);
+    const int zl = lane / LPR * NLD, zr = wave * WR + zl, zc = 4 * (lane % LPR);         // rows zr, zr + 1 ..
     const int cr = tid / CPR, cc = CPT * (tid % CPR);
     const bool c_on = k0 + cc < a.ldc;
     const int lb = a.ldc / 32;
@@ -136,13 +169,13 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
         if (FULL) {
             const long row = min(step * R, a.M - R);
             const int zcl = zc < a.N ? zc : 0, ccl = c_on ? cc : 0;
-            const unsigned oz = ((unsigned)zr * (unsigned)a.ldz + zcl) * 4u, oc = (unsigned)cr * (unsigned)a.ldc + ccl, ob = (unsigned)cr * (unsigned)lb + ccl / 32;
+            const unsigned oz = ((unsigned)zl * (unsigned)a.ldz + zcl) * 4u, oc = (unsigned)cr * (unsigned)a.ldc + ccl, ob = (unsigned)cr * (unsigned)lb + ccl / 32;
             const unsigned char *bc = a.codes + row * a.ldc + k0, *bb = a.bytes + row * lb + k0 / 32;
             T8_UNIFORM(bc);
             T8_UNIFORM(bb);
 #pragma unroll
             for (int i = 0; i < NLD; ++i) {
-                const float* p = a.dz + (row + i * RPL) * a.ldz;
+                const float* p = a.dz + (row + wave * WR + i) * a.ldz;
                 T8_UNIFORM(p);
                 dv[i] = t8_at<t8_v4<float>>(p, oz);
             }
@@ -151,7 +184,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
         }
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
-            const long r = step * R + zr + i * RPL;
+            const long r = step * R + zr + i;
             dv[i] = r < a.M ? t8_load4(a.dz + r * a.ldz + zc, a.N - zc) : t8_f4{0.f, 0.f, 0.f, 0.f};
         }
         const long r = step * R + cr;
@@ -208,45 +241,66 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             }
     }
     t8_f4 bsum = {0.f, 0.f, 0.f, 0.f};
-    int ze = 14, xe = 8;                                                      // bounds: dz is staged times 2^(140 - ze), codes times 2^(byte - xe + 5)
-    // ---- this lane's part of the step in its two images; true if something lies above the bounds
-    auto stage = [&](Step& B) -> bool {
-        float m = 0.f;
+    int ce = 28, tce[TB];                                                     // bounds on the products' exponents: of the lane's block of 32 columns, of the wave's dW
+#pragma unroll
+    for (int j = 0; j < TB; ++j) tce[j] = 28;
+    // ---- the exponents of this lane's rows of dz and, the last one, of the row that its codes belong to.  0: a row of zeros (what is not finite does not
+    // count); 14 at least otherwise, so that 2^(141 - e) is a number
+    auto measure = [&](int (&e)[NLD + 1]) {
+        auto rows = [&](bool finite) -> unsigned {
+            unsigned m[NLD];
+#pragma unroll
+            for (int i = 0; i < NLD; ++i) {
+                m[i] = 0u;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const unsigned b = __float_as_uint(dv[i][c]) & 0x7FFFFFFFu;
+                    m[i] = max(m[i], finite && b >= 0x7F800000u ? 0u : b);
+                }
+            }
+            return t8_row_max<NLD, LPR>(m, lane);
+        };
+        unsigned m = rows(false);
+        if (__any(m >= 0x7F800000u)) m = rows(true);
+        m = m == 0u ? 0u : max(m >> 23, 14u);
+        e[0] = (int)t8_dpp<0x00>(m), e[1] = (int)t8_dpp<0x55>(m);             // quad_perm 0 0 0 0, 1 1 1 1
+        if (NLD == 4) e[NLD - 2] = (int)t8_dpp<0xAA>(m), e[NLD - 1] = (int)t8_dpp<0xFF>(m);
+        const int p = lane / CPR % NLD;
+        e[NLD] = p & 1 ? e[1] : e[0];
+        if (NLD == 4) e[NLD] = p & 2 ? (p & 1 ? e[NLD - 1] : e[NLD - 2]) : e[NLD];
+    };
+    // ---- this lane's part of the step in its two images, under the bounds; of Swish: the values and derivatives
+    typedef t8_f4 Vals[ACT == ACT_SWISH ? CW : 1];
+    auto stage = [&](Step& B, const int (&e)[NLD + 1], const Vals& y, const Vals& dy) {
+        const int ec = e[NLD];
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
-            const float G = FULL && (zr + i * RPL < shift || zc >= a.N) ? 0.f : t8_pow2(267 - ze);
+            const float G = FULL && zc >= a.N ? 0.f : __uint_as_float((unsigned)(268 - e[i]) << 23);         // 2^(141 - e); of zeros: some number
             t8_u2 h, l;
             unsigned hw, lw;
-            m = fmaxf(fmaxf(fmaxf(m, fabsf(dv[i][0])), fabsf(dv[i][1])), fmaxf(fabsf(dv[i][2]), fabsf(dv[i][3])));
             split_f16_prod(dv[i][0], G, dv[i][1], G, hw, lw);
             h[0] = hw, l[0] = lw;
             split_f16_prod(dv[i][2], G, dv[i][3], G, hw, lw);
             h[1] = hw, l[1] = lw;
-            *reinterpret_cast<t8_u2*>(&B.z[0][zr + i * RPL][zc]) = h;
-            *reinterpret_cast<t8_u2*>(&B.z[1][zr + i * RPL][zc]) = l;
+            *reinterpret_cast<t8_u2*>(&B.z[0][zr + i][zc]) = h;
+            *reinterpret_cast<t8_u2*>(&B.z[1][zr + i][zc]) = l;
         }
-        const bool bad = bv == 255u;
+        if (cc == 0) B.e[cr] = ec;
         unsigned p[XPL][2 * CW];
         if (ACT == ACT_SWISH) {
-            const float up = t8_pow2(259 - xe);
+            const float up = ec ? t8_pow2(268 + ec - ce) : 0.f;               // (a row without a gradient: nothing of it counts)
 #pragma unroll
             for (int j = 0; j < CW; ++j) {
-                const t8_f4 v = t8_decode4<KIND>(cv[j], bv);
-                t8_f4 y, dy;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float d;
-                    y[i] = t8_swish(v[i], d);
-                    dy[i] = d;
-                }
-                split_f16_prod(y[0], up, y[1], up, p[0][2 * j], p[XPL - 1][2 * j]);
-                split_f16_prod(y[2], up, y[3], up, p[0][2 * j + 1], p[XPL - 1][2 * j + 1]);
-                *reinterpret_cast<t8_f4*>(&B.d[cr][cc + 4 * j]) = dy;
+                split_f16_prod(y[j][0], up, y[j][1], up, p[0][2 * j], p[XPL - 1][2 * j]);
+                split_f16_prod(y[j][2], up, y[j][3], up, p[0][2 * j + 1], p[XPL - 1][2 * j + 1]);
+                *reinterpret_cast<t8_f4*>(&B.d[cr][cc + 4 * j]) = dy[j];
             }
         } else {
             // byte c beside 0x64 is the fp16 number 1024 + c (signed: c + 128 after the sign bit is turned): times the power of two, less what it
-            // is too much - one fused multiply-add for two codes, exact
-            const _Float16 s = bad ? __builtin_bit_cast(_Float16, (unsigned short)0x7E00) : (_Float16)t8_pow2((int)bv - xe + 132);
+            // is too much - one fused multiply-add for two codes, exact down to 2^-24
+            const bool bad = bv == 255u;
+            const int k = min((int)bv + ec - ce, 0) + 5;
+            const _Float16 s = bad ? __builtin_bit_cast(_Float16, (unsigned short)0x7E00) : (_Float16)t8_pow2(k + 127);
             const _Float16 o = (KIND == T8_RELU ? (_Float16)-1024.0f : (_Float16)-1152.0f) * s;
             const t8_hp s2 = {s, s}, o2 = {o, o};
 #pragma unroll
@@ -255,6 +309,15 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                 p[0][2 * j] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(t8_hp, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)), s2, o2));
                 p[0][2 * j + 1] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(t8_hp, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)), s2, o2));
             }
+            // codes of smaller powers of two end among fp16's smallest numbers: each is rounded there by itself
+            if (__any(k < -24 && k >= -33 && !bad)) {
+                const float f = bad ? __uint_as_float(0x7FC00000u) : t8_pow2(k + 127);
+#pragma unroll
+                for (int j = 0; j < CW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        p[0][2 * j + i] = __builtin_bit_cast(unsigned, t8_hp{(_Float16)(t8_q<KIND>(cv[j], 2 * i) * f), (_Float16)(t8_q<KIND>(cv[j], 2 * i + 1) * f)});
+            }
         }
 #pragma unroll
         for (int q = 0; q < XPL; ++q)
@@ -262,30 +325,11 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             for (int j = 0; j < CPT / 8; ++j)
                 *reinterpret_cast<t8_u4*>(&B.x[q][cr][cc + 8 * j]) = t8_u4{p[q][4 * j], p[q][4 * j + 1], p[q][4 * j + 2], p[q][4 * j + 3]};
         if (ACT == ACT_RELU) *reinterpret_cast<t8_cw*>(&B.c[cr][cc / 4]) = cv;
-        return m >= t8_pow2(ze + 1) || (!bad && (int)bv > xe);
     };
     float* const wout = a.wpart + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * NP * KP;
     bool first = true;
     int it = 0;
     while (step < nsteps) {              // one stretch of steps under the same bounds
-        {
-            unsigned m = 0;
-#pragma unroll
-            for (int i = 0; i < NLD; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) m = max(m, t8_expo(dv[i][c]));
-            unsigned mx = bv == 255u ? 0u : bv;
-#pragma unroll
-            for (int o = 32; o; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o)), mx = max(mx, (unsigned)__shfl_xor((int)mx, o));
-            if (lane == 0) red[wave] = m | mx << 8;
-            wg_barrier();
-            m = mx = 0;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) m = max(m, red[w] & 0xFFu), mx = max(mx, red[w] >> 8);
-            ze = __builtin_amdgcn_readfirstlane((int)m > ze ? min((int)m + T8_ZROOM, 254) : ze);
-            xe = __builtin_amdgcn_readfirstlane((int)mx > xe ? (int)mx + T8_XROOM : xe);
-            if (tid < 2) flag[tid] = 0u;                                      // (everybody has read the flag that ended the last stretch)
-        }
         f32x4 accs[NBN][KB];                                                  // the stretch's sums: T8_FOLD steps at a time
 #pragma unroll
         for (int b = 0; b < NBN; ++b)
@@ -298,12 +342,57 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             for (int b = 0; b < NBN; ++b)
 #pragma unroll
                 for (int x = 0; x < KB; ++x) accw[b][x] = f32x4{0.f, 0.f, 0.f, 0.f};
-            // (a stretch's first step is what its bounds were made of: nothing to ask - and what is not finite would ask for more for ever)
             for (int k = 0; k < T8_FOLD && step < nsteps; ++k, step += gridDim.x, ++it, fresh = false) {
                 Step& B = sb[it & 1];
-                if (FULL) shift = (int)(step * R - min(step * R, a.M - R));
-                const bool over = stage(B);
-                if (!fresh && __any(over) && lane == 0) flag[it & 1] = 1u;
+                if (FULL) {
+                    shift = (int)(step * R - min(step * R, a.M - R));
+                    if (shift) {                                              // (the last step: rows that were done already count as zeros)
+#pragma unroll
+                        for (int i = 0; i < NLD; ++i)
+                            if (zr + i < shift) dv[i] = t8_f4{0.f, 0.f, 0.f, 0.f};
+                    }
+                }
+                int e[NLD + 1];
+                Vals y, dy;
+                measure(e);
+                // the exponent of the largest product of this lane's row of dz and its part of x (the values' own, or the tape's byte); 0: none
+                int c = bv == 0u || bv == 255u ? 0 : (int)bv;
+                if (ACT == ACT_SWISH) {
+                    unsigned top = 0u;
+#pragma unroll
+                    for (int j = 0; j < CW; ++j) {
+                        const t8_f4 v = t8_decode4<KIND>(cv[j], bv);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float d;
+                            y[j][i] = t8_swish(v[i], d);
+                            dy[j][i] = d;
+                            top = max(top, __float_as_uint(y[j][i]) & 0x7FFFFFFFu);
+                        }
+                    }
+                    c = top == 0u || top >= 0x7F800000u ? 0 : max((int)(top >> 23), 14);
+                }
+                c = c == 0 || e[NLD] == 0 ? 0 : c + e[NLD];
+                // a stretch's first step is what its bounds are made of
+                if (fresh) {
+                    int t = c;
+#pragma unroll
+                    for (int o = 1; o < 64; o = 2 * o == LB ? CPR : 2 * o) t = max(t, __shfl_xor(t, o));    // (the lanes of a block of columns)
+                    if (lane < CPR && !(lane % LB)) red[wave][lane / LB] = (unsigned)t;
+                    wg_barrier();
+                    auto bound = [&](int block, int now) {
+                        int u = 0;
+#pragma unroll
+                        for (int w = 0; w < NW; ++w) u = max(u, (int)red[w][block]);
+                        return u > now ? u + T8_ROOM(ACT) : now;
+                    };
+                    ce = bound(cc / 32, ce);
+#pragma unroll
+                    for (int j = 0; j < TB; ++j) tce[j] = __builtin_amdgcn_readfirstlane(bound(xf / 32 + j, tce[j]));
+                    if (tid < 2) flag[tid] = 0u;                              // (everybody has read the flag that ended the last stretch)
+                }
+                stage(B, e, y, dy);
+                if (!fresh && __any(c > ce) && lane == 0) flag[it & 1] = 1u;
                 wg_barrier();
                 if (!fresh && __builtin_amdgcn_readfirstlane((int)flag[it & 1])) {          // (the same for every wave)
                     same = false;
@@ -311,7 +400,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                 }
 #pragma unroll
                 for (int i = 0; i < NLD; ++i)
-                    if (!FULL || zr + i * RPL >= shift) bsum += dv[i];
+                    bsum += dv[i];
                 const long row0 = FULL ? min(step * R, a.M - R) : step * R;
                 const int done = shift;
                 asm volatile("" ::: "memory");
@@ -341,12 +430,12 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                     __builtin_amdgcn_sched_barrier(0);                                // (without these the reads of all parts move up and the registers run out)
                     // dx = act'(v) (dz W): lane = row n16 of the block of rows, features 4 q4 .. + 3 of the block of features
                     if (a.dx) {
-                        const int e = we + ze - 280;
                         float* const bx = a.dx + (row0 + wr + 16 * rp) * a.lddx + k0 + kf;
                         const unsigned ox = ((unsigned)n16 * (unsigned)a.lddx + 4 * q4) * 4u;
 #pragma unroll
                         for (int rb = 0; rb < RB; ++rb) {
                             const int lr = wr + 16 * (rp + rb) + n16;                 // row of the step
+                            const int e = we + B.e[lr] - 281;
 #pragma unroll
                             for (int b = 0; b < NBK; ++b) {
                                 const int f = kf + 16 * b + 4 * q4, k = k0 + f;
@@ -417,7 +506,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                     for (int i = 0; i < 4; ++i) {
                         float* o = wout + (nf + 16 * b + i) * KP + xf + 16 * x;
                         T8_UNIFORM(o);
-                        const float v = __builtin_amdgcn_ldexpf(accs[b][x][i], ze + xe - 272);
+                        const float v = __builtin_amdgcn_ldexpf(accs[b][x][i], tce[x / 2] - (ACT == ACT_SWISH ? 282 : 273));
                         t8_put<float>(o, ol, add ? t8_at<float>(o, ol) + v : v);
                     }
         };
@@ -429,11 +518,11 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
         float* s = reinterpret_cast<float*>(&sb[0]);
         wg_barrier();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[zr * NP + zc + i] = bsum[i];
+        for (int i = 0; i < 4; ++i) s[tid / LPR * NP + zc + i] = bsum[i];
         wg_barrier();
         if (tid < NP) {
             float t = 0.f;
-            for (int r = 0; r < RPL; ++r) t += s[r * NP + tid];
+            for (int r = 0; r < LANES / LPR; ++r) t += s[r * NP + tid];
             a.bpart[(size_t)blockIdx.x * NP + tid] = t;
         }
     }
