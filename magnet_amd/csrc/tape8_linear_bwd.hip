@@ -80,10 +80,11 @@ __device__ __forceinline__ t8_u2 t8_tr(const unsigned short* p) {
     return __builtin_bit_cast(t8_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) t8_s4*)(p)));
 }
 __device__ __forceinline__ t8_h8 t8_join(t8_u2 a, t8_u2 b) { return __builtin_bit_cast(t8_h8, t8_u4{a[0], a[1], b[0], b[1]}); }
-// e^-v (finite: past 87 both s and what is left of it are under 2^-125) and s = 1 / (1 + e^-v)
+// e^-v and s = 1 / (1 + e^-v), both finite.  Under -87, where e^-v nears the end of fp32, s is 0, and with it Swish and its derivative: what
+// either still is there lies under 2^-118
 __device__ __forceinline__ float t8_sigmoid(float v, float& e) {
     e = __expf(fminf(-v, 87.0f));
-    return __builtin_amdgcn_rcpf(1.0f + e);
+    return v < -87.0f ? 0.f : __builtin_amdgcn_rcpf(1.0f + e);
 }
 // Swish v s and its derivative s (1 + v (1 - s)) with 1 - s = e^-v s: no cancellation where s is near 1
 __device__ __forceinline__ float t8_swish(float v, float& d) {

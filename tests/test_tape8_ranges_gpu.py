@@ -166,3 +166,22 @@ def test_zero_rows_and_rows_that_are_not_finite():
         assert not any(o.any() for o in everything)
         tiny = torch.full_like(dz, 1e-44) * torch.randint(-3, 4, dz.shape, device="cuda")       # subnormal: multiples of 2^-149
         check_own(tiny, t, w, act, ops.tape8_linear_bwd(tiny, t, w, act))
+
+
+def test_far_arguments_of_swish():
+    """Swish and its derivative from the most negative argument that a tape holds to the largest: 0, v e^v on the way, v and 1"""
+    from magnet_amd import ops
+    for v0 in (-1e38, -1e34, -1e6, -1000.0, -200.0, -104.0, -90.0, -88.0, -87.0, -86.0, -60.0, -20.0, -1.25, -1e-3, 0.0, 1e-30, 0.7, 20.0, 90.0, 1e6, 1e34, 1e38):
+        x = torch.zeros(2, 32, device="cuda")
+        x[:, 3] = v0
+        t = ops.tape8_pack(x)
+        dz, w = torch.ones(2, 1, device="cuda"), torch.ones(1, 32, device="cuda")
+        dx, dW, _ = ops.tape8_linear_bwd(dz, t, w, "swish")
+        v = ref_values(t.codes, t.bytes, 32, "signed")[0, 3]
+        s, r = torch.sigmoid(v), torch.sigmoid(-v)
+        one = float(v * s * r)
+        # (the exponential's argument is off by 2^-23 of itself; under -87 the value, under 2^-118, is taken as 0)
+        rel = 2.0 ** -19 * (1 + min(abs(float(v)), 128.0) / 8)
+        assert abs(float(dx[0, 3]) - float(s + v * s * r)) <= rel * (float(s) + abs(one)) + 2.0 ** -118, v0
+        assert abs(float(dW[0, 3]) - 2 * float(v * s)) <= 2 * rel * abs(float(v * s)) + 2.0 ** -117, v0
+        assert v0 > -1e3 or (float(dx[0, 3]) == 0.0 and float(dW[0, 3]) == 0.0)
