@@ -548,11 +548,11 @@ int magnet_mpnn_edge_bwd_w_flags_f32(const float* A, const float* Bm, const floa
  *      models/backbones/mlp.py:9-28 in fp32.  A tape of M rows of W values: codes [M][32 ceil(W / 32)] (16-byte aligned) and one byte per
  *      block of 32 columns, bytes [M][ceil(W / 32)]; value = code 2^(byte - 127), byte 0 = zeros, 255 = NaN (the block held a value that is
  *      not finite).  kind 0 (signed): code = round(x / step) in [-127, 127]; kind 1 (behind a ReLU): 0 where x <= 0, else in [1, 255].
- *      dtype: 0 = fp32, 1 = bf16, 2 = fp16.  Row strides (ld*) count elements. ---- */
+ *      dtype: 0 = fp32, 1 = bf16, 2 = fp16.  Row strides (ld*) count elements.  Widths (W, N, K) < 2^31 - 255. ---- */
 int magnet_tape8_pack(const void* x, int dtype, long ldx, long M, int W, int kind, void* codes, void* bytes, void* stream);
 int magnet_tape8_unpack(const void* codes, const void* bytes, long M, int W, int kind, void* y, int dtype, long ldy, void* stream);
 /* A Linear y = x W^T + b walked back from the tape of its input (torch autograd of nn.Linear and its activation, models/backbones/mlp.py:9-28,
- * models/mpnn.py:15-24,81-90), any N, K >= 1: with v the tape's values and x = act(v)
+ * models/mpnn.py:15-24,81-90), any N, K >= 1 (a launch takes 4096 columns of K): with v the tape's values and x = act(v)
  *   dx [M][K] = act'(v) (dz W),  dW [N][K] (+)= dz^T x,  db [N] (+)= column sums of dz       (dx, db may be NULL)
  * act: MAGNET_ACT_NONE (signed tape of x), _RELU (relu tape of x: act' = x > 0), _SWISH (signed tape of Swish's argument).  dx must not
  * overlap dz.  M = 0 zeroes dW / db (accumulate == 0).  workspace: magnet_tape8_linear_bwd_workspace(M, N, K) floats. */

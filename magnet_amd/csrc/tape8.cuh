@@ -19,6 +19,7 @@ typedef unsigned t8_u4 __attribute__((ext_vector_type(4)));
 
 enum { T8_SIGNED = 0, T8_RELU = 1 };
 enum { T8_F32 = 0, T8_BF16 = 1, T8_F16 = 2 };
+#define T8_WIDEST (INT32_MAX - 255)      // columns are counted in 32 bits, up to the end of their block (of 128 in the Linear)
 
 // four neighbouring values of any alignment (the hardware takes 16-byte accesses at 4-byte, 8-byte ones at 2-byte addresses)
 template <typename T>

@@ -101,7 +101,7 @@ static int t8_unpack_as(const void* codes, const void* bytes, long M, int W, int
 }
 
 extern "C" int magnet_tape8_pack(const void* x, int dtype, long ldx, long M, int W, int kind, void* codes, void* bytes, void* stream) {
-    if (M < 0 || W < 1 || ldx < W || kind < 0 || kind > 1 || ((uintptr_t)codes & 15)) return -2;
+    if (M < 0 || W < 1 || W > T8_WIDEST || ldx < W || kind < 0 || kind > 1 || ((uintptr_t)codes & 15)) return -2;
     if (M == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
@@ -112,7 +112,7 @@ extern "C" int magnet_tape8_pack(const void* x, int dtype, long ldx, long M, int
     return -2;
 }
 extern "C" int magnet_tape8_unpack(const void* codes, const void* bytes, long M, int W, int kind, void* y, int dtype, long ldy, void* stream) {
-    if (M < 0 || W < 1 || ldy < W || kind < 0 || kind > 1 || ((uintptr_t)codes & 15)) return -2;
+    if (M < 0 || W < 1 || W > T8_WIDEST || ldy < W || kind < 0 || kind > 1 || ((uintptr_t)codes & 15)) return -2;
     if (M == 0) return 0;
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {

@@ -44,6 +44,7 @@ struct T8LinArgs {
     float* bpart;                        // [gridDim.x][NP] partial sums of db
     long M, ldz, ldw, lddx;
     int N, K, ldc, exact, add_dx;        // exact: N = NP and K a multiple of KP; add_dx: dx += (a later block of N)
+    int kb0;                             // the launch's first block of K
 };
 
 template <int CTRL>
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     __shared__ unsigned red[NW][CB], flag[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, q4 = lane >> 4;
-    const int k0 = blockIdx.y * KP;
+    const int k0 = (a.kb0 + blockIdx.y) * KP;
     const int kf = 16 * NBK * (wave % KW), wr = (wave / KW) * (R / RW);       // its features and rows of dx
     const int nf = 16 * NBN * (wave % NG), xf = 16 * KB * (wave / NG);        // its features of dz and of x in dW
     // ---- what this lane loads of a step
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
         else sums(true);
         first = false;
     }
-    if (blockIdx.y == 0) {                                                    // the lanes that hold the same columns of dz, in order
+    if (a.kb0 + blockIdx.y == 0) {                                            // the lanes that hold the same columns of dz, in order
         float* s = reinterpret_cast<float*>(&sb[0]);
         wg_barrier();
 #pragma unroll
@@ -530,12 +531,13 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
 }
 
 // dW[n][k] (+)= sum over the workgroups of their partial sums, in order: a workgroup takes 64 neighbouring sums, its sixteen waves a run of the
-// partials each (short chains: the reads' latency is what this kernel takes, and the sums' rounding grows with their length).  blockIdx.y = block of K; the last one: db
+// partials each (short chains: the reads' latency is what this kernel takes, and the sums' rounding grows with their length).  blockIdx.y = block of K of
+// the launch, which begins at block kb0; one more, in the first launch: db
 __global__ void __launch_bounds__(1024) k_tape8_linear_sum(const float* __restrict__ wpart, const float* __restrict__ bpart, int nwg, int NP, int KP, int N, int K,
-                                                          float* __restrict__ dW, long lddw, float* __restrict__ db, int add) {
+                                                          int kb0, int kbn, float* __restrict__ dW, long lddw, float* __restrict__ db, int add) {
     __shared__ float s[16][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const bool bias = blockIdx.y == gridDim.y - 1;
+    const bool bias = blockIdx.y == kbn;
     const int o = blockIdx.x * 64 + lane, n_out = bias ? NP : NP * KP;
     if (blockIdx.x * 64 >= n_out) return;
     const float* p = bias ? bpart : wpart + (size_t)blockIdx.y * nwg * NP * KP;
@@ -548,7 +550,7 @@ __global__ void __launch_bounds__(1024) k_tape8_linear_sum(const float* __restri
     if (wave) return;
 #pragma unroll
     for (int w = 1; w < 16; ++w) t += s[w][lane];
-    const int n = bias ? o : o / KP, k = bias ? 0 : blockIdx.y * KP + o % KP;
+    const int n = bias ? o : o / KP, k = bias ? 0 : (kb0 + blockIdx.y) * KP + o % KP;
     if (n >= N || k >= K) return;
     float* d = bias ? db + n : dW + n * lddw + k;
     if (bias && !db) return;
@@ -562,6 +564,7 @@ static unsigned t8_fill_grid(long n) { return (unsigned)(n < (1l << 28) ? (n + 2
 
 #define T8_BLOCK 128
 static int t8_pad(int n) { return n <= 64 ? 64 : 128; }                       // a block of at most 128 features, as 64 or 128
+#define T8_KBLOCKS 32                         // blocks of K of a launch: the partial sums of more would take memory without end (200 000 columns: 13 GB)
 // one workgroup a CU of eight waves, two (three) of four; fewer where K has several blocks
 static int t8_lin_grid(long M, int np, int kp, int kblocks, int act) {
     const int R = T8_ROWS(np, kp, act);
@@ -570,9 +573,9 @@ static int t8_lin_grid(long M, int np, int kp, int kblocks, int act) {
 }
 
 extern "C" int magnet_tape8_linear_bwd_workspace(long M, long N, long K, long* floats) {
-    if (M < 0 || N < 1 || K < 1 || N > INT32_MAX || K > INT32_MAX) return -2;
-    const int kp = t8_pad((int)K), kb = (int)((K + kp - 1) / kp), np = t8_pad((int)N);
-    *floats = (long)t8_lin_grid(M, np, kp, kb, ACT_SWISH) * ((long)np * kp * kb + np);      // (most workgroups: steps of 32 rows)
+    if (M < 0 || N < 1 || K < 1 || N > T8_WIDEST || K > T8_WIDEST) return -2;
+    const int kp = t8_pad((int)K), kb = (int)((K + kp - 1) / kp), np = t8_pad((int)N), kbn = kb < T8_KBLOCKS ? kb : T8_KBLOCKS;
+    *floats = (long)t8_lin_grid(M, np, kp, kb, ACT_SWISH) * ((long)np * kp * kbn + np);     // (most workgroups: steps of 32 rows)
     return 0;
 }
 
@@ -593,7 +596,8 @@ static void t8_lin_shape(const T8LinArgs& a, int np, int kp, int act, dim3 grid,
 extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void* codes, const void* bytes, const float* w, long ldw, long M, int N, int K,
                                            int act, float* dx, long lddx, float* dW, long lddw, float* db, int accumulate, float* workspace,
                                            void* stream) {
-    if (M < 0 || N < 1 || K < 1 || ldz < N || ldw < K || lddw < K || (dx && lddx < K) || act < 0 || act > 2 || !dW || ((uintptr_t)codes & 15)) return -2;
+    if (M < 0 || N < 1 || K < 1 || ldz < N || ldw < K || lddw < K || (dx && lddx < K) || act < 0 || act > 2 || !dW || ((uintptr_t)codes & 15) || N > T8_WIDEST || K > T8_WIDEST)
+        return -2;
     hipStream_t st = (hipStream_t)stream;
     if (M == 0) {
         if (!accumulate) {
@@ -603,23 +607,27 @@ extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void
         return (int)hipGetLastError();
     }
     const int kp = t8_pad(K), kb = (K + kp - 1) / kp;
-    const int np = t8_pad(N);
-    const dim3 grid(t8_lin_grid(M, np, kp, kb, act), kb);
+    const int np = t8_pad(N), wgs = t8_lin_grid(M, np, kp, kb, act);
     for (int n0 = 0; n0 < N; n0 += T8_BLOCK) {
         const int n = N - n0 < T8_BLOCK ? N - n0 : T8_BLOCK;
         T8LinArgs a;
         a.dz = dz + n0, a.codes = (const unsigned char*)codes, a.bytes = (const unsigned char*)bytes, a.w = w + n0 * ldw, a.dx = dx;
-        a.wpart = workspace, a.bpart = workspace + (size_t)grid.x * np * kp * kb;
+        a.wpart = workspace, a.bpart = workspace + (size_t)wgs * np * kp * (kb < T8_KBLOCKS ? kb : T8_KBLOCKS);
         a.M = M, a.ldz = ldz, a.ldw = ldw, a.lddx = lddx, a.N = n, a.K = K, a.ldc = (K + 31) / 32 * 32;
         a.exact = n == np && !(K % kp);
         a.add_dx = n0 > 0;
         // (32-bit byte offsets inside a step of 32 rows)
         const bool full = M >= 64 && N <= T8_BLOCK && !(n & 3) && !(K & 3) && ldz < (1l << 24) && lddx < (1l << 24) && ldw < (1l << 24);
-        if (full) t8_lin_shape<true>(a, np, kp, act, grid, st);
-        else t8_lin_shape<false>(a, np, kp, act, grid, st);
-        k_tape8_linear_sum<<<dim3((np * kp + 63) / 64, kb + 1), 1024, 0, st>>>(a.wpart, a.bpart, grid.x, np, kp, n, K, dW + n0 * lddw, lddw, db ? db + n0 : nullptr, accumulate);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return (int)e;
+        for (a.kb0 = 0; a.kb0 < kb; a.kb0 += T8_KBLOCKS) {
+            const int kbn = kb - a.kb0 < T8_KBLOCKS ? kb - a.kb0 : T8_KBLOCKS;
+            const dim3 grid(wgs, kbn);
+            if (full) t8_lin_shape<true>(a, np, kp, act, grid, st);
+            else t8_lin_shape<false>(a, np, kp, act, grid, st);
+            k_tape8_linear_sum<<<dim3((np * kp + 63) / 64, kbn + (a.kb0 == 0)), 1024, 0, st>>>(a.wpart, a.bpart, wgs, np, kp, n, K, a.kb0, kbn, dW + n0 * lddw, lddw,
+                                                                                            db ? db + n0 : nullptr, accumulate);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return (int)e;
+        }
     }
     return 0;
 }

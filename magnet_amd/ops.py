@@ -804,6 +804,7 @@ TAPE8_KINDS = {"signed": 0, "relu": 1}
 _T8_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _T8_ACTS = {"none": ACT_NONE, "relu": ACT_RELU, "swish": ACT_SWISH}
 NORM_JOIN_MAX_WIDTH = 4096
+TAPE8_MAX_WIDTH = 2 ** 31 - 256          # (kernels count columns in 32 bits)
 
 
 @dataclass
@@ -824,7 +825,7 @@ class Tape8:
 
 def tape8_empty(rows: int, width: int, kind: str = "signed", device="cuda") -> Tape8:
     """an uninitialised tape (``tape8_pack(out=...)``)"""
-    if kind not in TAPE8_KINDS or width < 1 or rows < 0:
+    if kind not in TAPE8_KINDS or not 1 <= width <= TAPE8_MAX_WIDTH or rows < 0:
         raise ValueError(f"magnet_amd: no 8-bit tape of kind {kind!r}, {rows} rows, width {width}")
     nb = (width + 31) // 32
     return Tape8(torch.empty(rows, 32 * nb, dtype=torch.uint8, device=device), torch.empty(rows, nb, dtype=torch.uint8, device=device), width, kind)
@@ -834,7 +835,7 @@ def _tape8_ok(t: Tape8, name="tape", kind=None, width=None, rows=None) -> Tape8:
     if not isinstance(t, Tape8):
         raise TypeError(f"magnet_amd: {name} must be an ops.Tape8 (got {type(t).__name__})")
     nb = (t.width + 31) // 32
-    if t.kind not in TAPE8_KINDS or t.width < 1:
+    if t.kind not in TAPE8_KINDS or not 1 <= t.width <= TAPE8_MAX_WIDTH:
         raise ValueError(f"magnet_amd: {name}: kind {t.kind!r}, width {t.width}")
     c, b = t.codes, t.bytes
     _is_tensor(c, name)
@@ -881,6 +882,8 @@ def _matrix(t, name, dtypes, shape=None):
     s = tuple(t.shape)
     if len(s) != 2 or s[1] < 1 or (shape is not None and s != shape):
         raise ValueError(f"magnet_amd: {name} has shape {s}" + (f", expected {shape}" if shape is not None else ", expected [rows, width >= 1]"))
+    if s[1] > TAPE8_MAX_WIDTH:
+        raise ValueError(f"magnet_amd: {name} {s}: at most {TAPE8_MAX_WIDTH} columns")
     if not t.is_contiguous():
         st = t.stride()
         if (st[1] != 1 and s[1] > 1) or (s[0] > 1 and st[0] < s[1]):

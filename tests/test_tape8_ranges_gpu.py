@@ -185,3 +185,32 @@ def test_far_arguments_of_swish():
         assert abs(float(dx[0, 3]) - float(s + v * s * r)) <= rel * (float(s) + abs(one)) + 2.0 ** -118, v0
         assert abs(float(dW[0, 3]) - 2 * float(v * s)) <= 2 * rel * abs(float(v * s)) + 2.0 ** -117, v0
         assert v0 > -1e3 or (float(dx[0, 3]) == 0.0 and float(dW[0, 3]) == 0.0)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_a_very_wide_weight(act):
+    """more than 65 536 blocks of columns; and a workspace that does not grow with the width"""
+    from magnet_amd import ops
+    K = 65536 * 128 + 261
+    t = ops.tape8_pack(torch.randn(3, K, device="cuda"), "relu" if act == "relu" else "signed")
+    dz, w = torch.randn(3, 2, device="cuda"), torch.randn(2, K, device="cuda")
+    dx, dW, db = ops.tape8_linear_bwd(dz, t, w, act)
+    for a in (0, 4096 - 32, 65535 * 128, K // 32 * 32 - 4096):     # pieces of it, from blocks of 32 columns
+        b = min(a + 4200, K)
+        part = ops.Tape8(t.codes[:, a:(b + 31) // 32 * 32].contiguous(), t.bytes[:, a // 32:(b + 31) // 32].contiguous(), b - a, t.kind)
+        want = ops.tape8_linear_bwd(dz, part, w[:, a:b], act)
+        assert torch.allclose(dx[:, a:b], want[0], rtol=1e-5, atol=1e-5) and torch.allclose(dW[:, a:b], want[1], rtol=1e-5, atol=1e-5) and torch.equal(db, want[2])
+        check_own(dz, part, w[:, a:b], act, want)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_weights_wider_than_one_launch(act):
+    from magnet_amd import ops
+    dz, t, w = linear_case(200, 5, 9000, act, seed=1)
+    got = ops.tape8_linear_bwd(dz, t, w, act)
+    check_own(dz, t, w, act, got)
+    dW, db = torch.ones_like(got[1]), torch.ones_like(got[2])
+    ops.tape8_linear_bwd(dz, t, w, act, dW=dW, db=db, accumulate=True)
+    assert torch.equal(dW, 1 + got[1]) and torch.equal(db, 1 + got[2])
+    dz, t, w = linear_case(70, 131, 8300, act, seed=2)
+    check_own(dz, t, w, act, ops.tape8_linear_bwd(dz, t, w, act))
