@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 import types
 
 import torch
@@ -38,7 +39,26 @@ BWD_GEMM = "bf16x6"
 DIRECT_SRC_GRAD = __import__("os").environ.get("MAGNET_DIRECT_SRC_GRAD", "1") != "0"
 # MAGNET_ACCUM_PARAM_GRADS=0 (development A/B): see accumulate_param_grads
 ACCUM_PARAM_GRADS = __import__("os").environ.get("MAGNET_ACCUM_PARAM_GRADS", "1") != "0"
-_ACCUM = {"on": False}
+
+
+class _Switch(threading.local):
+    """whether a training scope is open in this thread, and what was before each one that is (a model that trains in another thread has its own)"""
+
+    def __init__(self):
+        self.on, self.before = False, []
+
+    def __getitem__(self, key):
+        return getattr(self, key)
+
+    def enter(self, on):
+        self.before.append(self.on)
+        self.on = on
+
+    def leave(self):
+        self.on = self.before.pop()
+
+
+_ACCUM = _Switch()
 
 
 def in_ddp_forward() -> bool:
@@ -71,35 +91,33 @@ class accumulate_param_grads:
     parameter that carries a hook is always handed to autograd (``takes_inplace_grad``)."""
 
     def __enter__(self):
-        self.prev = _ACCUM["on"]
-        _ACCUM["on"] = ACCUM_PARAM_GRADS and not in_ddp_forward()
+        _ACCUM.enter(ACCUM_PARAM_GRADS and not in_ddp_forward())
         return self
 
     def __exit__(self, *exc):
-        _ACCUM["on"] = self.prev
+        _ACCUM.leave()
         return False
 
 
-_TAPE8 = {"on": False}
+_TAPE8 = _Switch()
 
 
 class tape8:
     """``with tape8():`` around the forward of a training step: the MLP chains built inside keep their tape in 8 bits (ops.Tape8) - every
     hidden activation as codes that carry the ReLU mask exactly, the normalised row in place of the LayerNorm's input - and their
     backward walks the hidden Linears back from it (ops.tape8_linear_bwd).  A quarter of the memory between forward and backward, and gradients of
-    the same function with activations rounded to a step of at most 2 / 255 of their block's largest value.  ``tape8(False)``: off inside."""
+    the same function with activations rounded to a step of at most 2 / 255 of their block's largest value.  ``tape8(False)``: off inside.  Like
+    ``torch.no_grad`` it holds for the thread that enters it."""
 
     def __init__(self, on=True):
         self.on = bool(on)
-        self.prev = []
 
     def __enter__(self):
-        self.prev.append(_TAPE8["on"])
-        _TAPE8["on"] = self.on
+        _TAPE8.enter(self.on)
         return self
 
     def __exit__(self, *exc):
-        _TAPE8["on"] = self.prev.pop()
+        _TAPE8.leave()
         return False
 
 
@@ -1007,7 +1025,7 @@ def mlp(M, groups, pk, params, *, epi=ops.EPI_STORE, res=None, csr=None, out_row
         M=int(M), tiles=tiles, runs=runs, pk=pk, epi=epi, n_src=len(srcs), n_par=len(params), has_res=res is not None,
         tgt=csr.tgt if csr is not None else None, rowptr=csr.rowptr if csr is not None else None,
         out_rows=int(out_rows if out_rows is not None else M), first_cols=first_cols, col_map=getattr(pk, "col_map", None),
-        inv_cache={}, final_relu=bool(final_relu), grad_chain=grad_chain, accum=_ACCUM["on"], tape8=_TAPE8["on"])
+        inv_cache={}, final_relu=bool(final_relu), grad_chain=grad_chain, accum=_ACCUM.on, tape8=_TAPE8.on)
     assert not (final_relu and (pk.ln is not None or epi != ops.EPI_STORE))
     srcs = [ops._f32(s, "mlp source") for s in srcs]
     extra = [ops._f32(res, "residual")] if res is not None else []

@@ -1,10 +1,12 @@
-"""The 8-bit tape's operators on any machine: what they refuse at the ends of their ranges, and what their workspaces take."""
+"""The 8-bit tape's operators on any machine: what they refuse at the ends of their ranges, what their workspaces take, and where the
+training scopes hold."""
 import ctypes as C
+import threading
 
 import pytest
 import torch
 
-from magnet_amd import _lib, ops
+from magnet_amd import _lib, autograd as AG, ops
 
 
 def test_widths_beyond_32_bits_are_refused():
@@ -32,3 +34,51 @@ def test_the_workspace_of_a_wide_weight():
             assert 0 < 4 * n.value <= 512 << 20, (M, K, n.value)
     assert entry(C.c_long(1), C.c_long(1), C.c_long((1 << 31) - 1), C.byref(n)) == -2
     assert entry(C.c_long(1), C.c_long((1 << 31) - 1), C.c_long(1), C.byref(n)) == -2
+
+
+@pytest.mark.parametrize("scope,state", [(lambda: AG.tape8(), lambda: AG._TAPE8["on"]), (lambda: AG.accumulate_param_grads(), lambda: AG._ACCUM["on"])])
+def test_a_training_scope_belongs_to_its_thread(scope, state, monkeypatch):
+    """a thread that trains beside one inside the scope does not see it, and threads that enter and leave overlapping leave it off"""
+    monkeypatch.setattr(AG, "ACCUM_PARAM_GRADS", True)
+    seen, steps = {}, [threading.Event() for _ in range(3)]
+
+    def first():
+        with scope():
+            steps[0].set()
+            steps[1].wait(10)
+            seen["first"] = state()
+        steps[2].set()
+
+    def second():
+        steps[0].wait(10)
+        seen["before"] = state()
+        with scope():
+            steps[1].set()
+            steps[2].wait(10)
+            seen["second"] = state()
+        seen["after"] = state()
+    threads = [threading.Thread(target=f) for f in (first, second)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(20)
+    assert seen == {"first": True, "before": False, "second": True, "after": False}
+    assert not state()
+
+
+def test_one_scope_object_in_two_threads():
+    both, inside, leave, after = AG.tape8(), threading.Event(), threading.Event(), []
+
+    def other():
+        with AG.tape8(False), both:
+            inside.set()
+            leave.wait(10)
+        after.append(AG._TAPE8["on"])
+    t = threading.Thread(target=other)
+    with both:
+        t.start()
+        inside.wait(10)
+    assert not AG._TAPE8["on"]
+    leave.set()
+    t.join(20)
+    assert after == [False]
