@@ -427,7 +427,7 @@ class _Mlp(torch.autograd.Function):
         # one more launch of the chain in the backward
         tape = ()
         K0 = len(m.tiles) * 32
-        wants_tape = nl > 1 and not m.final_relu and pk.layers[0][0].dtype in (torch.float16, torch.int16) and m.M > 0 and \
+        wants_tape = m.grad and nl > 1 and not m.final_relu and pk.layers[0][0].dtype in (torch.float16, torch.int16) and m.M > 0 and \
             any(ctx.needs_input_grad[1:])
         if wants_tape:
             # (no x0 at all when every k tile is factored or a dense copy of a source: an empty placeholder keeps the tuple's layout)
@@ -1025,7 +1025,8 @@ def mlp(M, groups, pk, params, *, epi=ops.EPI_STORE, res=None, csr=None, out_row
         M=int(M), tiles=tiles, runs=runs, pk=pk, epi=epi, n_src=len(srcs), n_par=len(params), has_res=res is not None,
         tgt=csr.tgt if csr is not None else None, rowptr=csr.rowptr if csr is not None else None,
         out_rows=int(out_rows if out_rows is not None else M), first_cols=first_cols, col_map=getattr(pk, "col_map", None),
-        inv_cache={}, final_relu=bool(final_relu), grad_chain=grad_chain, accum=_ACCUM.on, tape8=_TAPE8.on)
+        inv_cache={}, final_relu=bool(final_relu), grad_chain=grad_chain, accum=_ACCUM.on, tape8=_TAPE8.on,
+        grad=torch.is_grad_enabled())                      # (inside the Function it is off, and parameters ask for gradients under no_grad too)
     assert not (final_relu and (pk.ln is not None or epi != ops.EPI_STORE))
     srcs = [ops._f32(s, "mlp source") for s in srcs]
     extra = [ops._f32(res, "residual")] if res is not None else []
@@ -1041,7 +1042,7 @@ class _NormJoin(torch.autograd.Function):
         post = (post_g, post_b) if post_g is not None else None
         pre = (pre_g, pre_b) if pre_g is not None else None
         r = ops.norm_join(x, f, post=post, pre=pre, gate=gate, scale=meta.scale if scale is None else scale, norm=meta.norm, eps=meta.eps,
-                          tape=any(ctx.needs_input_grad[1:]))
+                          tape=meta.grad and any(ctx.needs_input_grad[1:]))
         ctx.meta = meta
         if r.post_tape is not None:
             pt, qt = r.post_tape, r.pre_tape
@@ -1070,7 +1071,7 @@ def norm_join(x, f, *, post=None, pre=None, gate=None, scale=1.0, norm="layer", 
     if gate is not None and isinstance(gate, torch.Tensor) and gate.dim() == 1:
         gate = gate.unsqueeze(0)
     vec = scale if isinstance(scale, torch.Tensor) else None
-    meta = types.SimpleNamespace(scale=None if vec is not None else float(scale), norm=norm, eps=float(eps))
+    meta = types.SimpleNamespace(scale=None if vec is not None else float(scale), norm=norm, eps=float(eps), grad=torch.is_grad_enabled())
     y, h = _NormJoin.apply(meta, x, f, gate, vec, post_g, post_b, pre_g, pre_b)
     return y, h
 

@@ -82,3 +82,19 @@ def test_one_scope_object_in_two_threads():
     leave.set()
     t.join(20)
     assert after == [False]
+
+
+def test_norm_join_keeps_a_tape_only_where_gradients_are_recorded(monkeypatch):
+    asked = []
+
+    def fake(x, f, *, tape, **kw):
+        asked.append(tape)
+        return ops.NormJoin(x + f, None)
+    monkeypatch.setattr(ops, "norm_join", fake)
+    x, gain = torch.randn(4, 8), torch.nn.Parameter(torch.ones(8))
+    with torch.no_grad():
+        AG.norm_join(x, x, post=(gain, None))
+    assert asked == [False]
+    AG.norm_join(x, x, post=(gain, None))
+    AG.norm_join(x, x, post=(gain.detach(), None))
+    assert asked == [False, True, False]
