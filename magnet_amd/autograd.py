@@ -1066,8 +1066,7 @@ class _NormJoin(torch.autograd.Function):
 def norm_join(x, f, *, post=None, pre=None, gate=None, scale=1.0, norm="layer", eps=1e-5):
     """differentiable ``ops.norm_join`` -> (y, h): y = x + scale * gate * post(f), h = pre(y) (None without ``pre``).  Gradients of x, f, gate,
     scale (a tensor) and the norms' gains and biases; between forward and backward only the normalised rows stay, in 8 bits."""
-    post_g, post_b = post if post is not None else (None, None)
-    pre_g, pre_b = pre if pre is not None else (None, None)
+    (post_g, post_b), (pre_g, pre_b) = ops.norm_pair(post, "post"), ops.norm_pair(pre, "pre")
     if gate is not None and isinstance(gate, torch.Tensor) and gate.dim() == 1:
         gate = gate.unsqueeze(0)
     vec = scale if isinstance(scale, torch.Tensor) else None

@@ -1038,12 +1038,18 @@ def _vector(t, name, W):
     return t.contiguous()
 
 
-def _norm_pair(p, name, W):
+def norm_pair(p, name):
+    """(gain, bias) of a norm, (None, None) of no norm"""
     if p is None:
         return None, None
     if not isinstance(p, (tuple, list)) or len(p) != 2 or p[0] is None:
         raise ValueError(f"magnet_amd: {name} is (gain, bias) with bias None where there is none")
-    return _vector(p[0], name + " gain", W), _vector(p[1], name + " bias", W)
+    return p[0], p[1]
+
+
+def _norm_pair(p, name, W):
+    g, b = norm_pair(p, name)
+    return _vector(g, name + " gain", W), _vector(b, name + " bias", W)
 
 
 def _join_args(x, name, post, pre, gate, scale, norm):

@@ -98,3 +98,12 @@ def test_norm_join_keeps_a_tape_only_where_gradients_are_recorded(monkeypatch):
     AG.norm_join(x, x, post=(gain, None))
     AG.norm_join(x, x, post=(gain.detach(), None))
     assert asked == [False, True, False]
+
+
+@pytest.mark.parametrize("side", ["post", "pre"])
+def test_norm_join_refuses_a_norm_without_a_gain(side):
+    """(as ops.norm_join does: a bias without a gain is no norm of this kind, not an absent one)"""
+    x, v = torch.randn(4, 8), torch.ones(8)
+    for bad in ((None, v), (None, None), (v,), (v, v, v), v):
+        with pytest.raises(ValueError, match=side):
+            AG.norm_join(x, x, **{side: bad})
