@@ -24,8 +24,8 @@
 // with its write; behind the barrier that the step has anyway all waves see it, add their sums so far to the workgroup's partial sums in
 // memory and begin again under a new bound (with a few binades to spare): rare after the first step, and nobody waits for a maximum
 // otherwise.  (Scaling the sums in registers instead costs a second set of them: measured as spills.)  A row's largest value is a few lane
-// permutes, and the wave that stages a row of dz stages its codes too, so the exponent never waits for another wave.  A wave scales its part
-// of W likewise, by the part's largest value.
+// permutes, and the wave that stages a row of dz stages its codes too, so the exponent never waits for another wave.  W's columns
+// have a scale each as well, by their largest value in the block of 128 rows: dx of one owes nothing to the others.
 #include "common.cuh"
 #include "split_single.cuh"
 #include "tape8.cuh"
@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     load(step);
     // ---- the wave's features of W^T: A operands (lane = feature of x, register j of k group q4 = feature 32 t + 8 q4 + j of dz)
     t8_h8 wh[NBK][NT], wl[NBK][NT];
-    int we;                                                                   // W is staged times 2^(140 - we): max |W| -> [2^13, 2^14)
+    unsigned we[NBK];                                                         // a feature of x is staged times 2^(140 - its exponent): max |W| over dz -> [2^13, 2^14);
+                                                                              // those of features 4 q4 .. + 3 of a block, a byte each (what the lane gets of dx)
     {
         auto w_at = [&](int b, int t, int j) -> float {
             const int n = 32 * t + 8 * q4 + j, k = k0 + kf + 16 * b + n16;
@@ -217,19 +218,16 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) wv[b][t][j] = w_at(b, t, j);
-        unsigned et = 0;
 #pragma unroll
-        for (int b = 0; b < NBK; ++b)
+        for (int b = 0; b < NBK; ++b) {
+            unsigned et = 14;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) et = max(et, t8_expo(wv[b][t][j]));
-#pragma unroll
-        for (int o = 32; o; o >>= 1) et = max(et, (unsigned)__shfl_xor((int)et, o));
-        we = max(__builtin_amdgcn_readfirstlane((int)et), 14);
-        const float s = t8_pow2(267 - we);
-#pragma unroll
-        for (int b = 0; b < NBK; ++b)
+            et = max(et, (unsigned)__shfl_xor((int)et, 16));
+            et = max(et, (unsigned)__shfl_xor((int)et, 32));
+            const float s = t8_pow2(267 - (int)et);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 t8_u4 h, l;
@@ -241,6 +239,10 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                 }
                 wh[b][t] = __builtin_bit_cast(t8_h8, h), wl[b][t] = __builtin_bit_cast(t8_h8, l);
             }
+            we[b] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) we[b] |= (unsigned)__shfl((int)et, 4 * q4 + i) << (8 * i);
+        }
     }
     t8_f4 bsum = {0.f, 0.f, 0.f, 0.f};
     int ce = 28, tce[TB];                                                     // bounds on the products' exponents: of the lane's block of 32 columns, of the wave's dW
@@ -437,13 +439,15 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
 #pragma unroll
                         for (int rb = 0; rb < RB; ++rb) {
                             const int lr = wr + 16 * (rp + rb) + n16;                 // row of the step
-                            const int e = we + B.e[lr] - 281;
+                            const int e = B.e[lr] - 281;
 #pragma unroll
                             for (int b = 0; b < NBK; ++b) {
                                 const int f = kf + 16 * b + 4 * q4, k = k0 + f;
                                 t8_f4 v;
+                                unsigned wb = we[b];
+                                asm volatile("" : "+v"(wb));                          // (or the four bytes are kept apart in registers across the loop)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(acc[b][rb][i], e);
+                                for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(acc[b][rb][i], e + (int)(wb >> (8 * i) & 0xFFu));
                                 if (ACT == ACT_RELU) {
                                     const unsigned w = B.c[lr][f / 4];
 #pragma unroll

@@ -15,8 +15,8 @@ def own_ref(dz, t, w, act):
     """(dx, dW, db) in 64 bits and a bound for each value, from the magnitudes that it is made of.
 
     dz goes as two fp16 pieces of dz 2^s with the row's largest magnitude in [2^14, 2^15): rounding the high piece leaves 2^-11, rounding
-    the low one 2^-11 of that, or half of fp16's smallest number, 2^-25 against 2^14: 2^-39 of the row's largest.  w likewise, its largest
-    (of the part of w that a wave holds) from 2^13: 2^-38 of it.  The product of the low pieces is left out: 2^-22.  Together under 2^-20 of |dz| |w|.
+    the low one 2^-11 of that, or half of fp16's smallest number, 2^-25 against 2^14: 2^-39 of the row's largest.  w likewise, a column's
+    largest from 2^13: 2^-38 of it.  The product of the low pieces is left out: 2^-22.  Together under 2^-20 of |dz| |w|.
     A sum of n terms in fp32 is off by n 2^-24 of the sum of magnitudes, three products a term.
     dW: the tape's values enter times a power of two that puts the largest product of a row's largest dz and its block's step at code 2^5 or up
     to 2^3 below (room for larger ones): codes 2^25 and more below that largest product lose what lies under 2^-25 there: with |dz| of the row
@@ -40,7 +40,7 @@ def own_ref(dz, t, w, act):
     tops = z.abs().amax(1, keepdim=True)
     s = z.abs() @ wd.abs()
     dx = d * (z @ wd)
-    bx = (d.abs() * ((2.0 ** -20 + 3 * N * 2.0 ** -24) * s + 2.0 ** -39 * tops * wd.abs().sum(0) + 2.0 ** -38 * wd.abs().max() * z.abs().sum(1, keepdim=True))
+    bx = (d.abs() * ((2.0 ** -20 + 3 * N * 2.0 ** -24) * s + 2.0 ** -39 * tops * wd.abs().sum(0) + 2.0 ** -38 * wd.abs().amax(0) * z.abs().sum(1, keepdim=True))
           + ed * s + 2.0 ** -20 * ed * s + 2.0 ** -126)
     if act == "swish":
         step = torch.stack([x[:, c:c + 32].abs().amax(1) for c in range(0, t.width, 32)], 1).repeat_interleave(32, 1)[:, :t.width]
@@ -106,6 +106,21 @@ def test_a_block_of_columns_of_dw_is_its_own(act, M, N, K):
     x = torch.randn(M, K, device="cuda") * torch.exp2(far + torch.randn(M, 1, device="cuda"))
     t = ops.tape8_pack(x, "relu" if act == "relu" else "signed")
     check_own(dz, t, w, act, ops.tape8_linear_bwd(dz, t, w, act))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M,N,K", [(300, 128, 128), (300, 64, 64), (200, 96, 200), (31, 33, 40), (70, 200, 100)])
+def test_a_column_of_dx_is_its_own(act, M, N, K):
+    """columns of the weight 2^60 apart, neighbours among them: each column of dx has the bits that it has beside others of its own size"""
+    from magnet_amd import ops
+    dz, t, w = linear_case(M, N, K, act, seed=N)
+    w = w * torch.exp2(torch.randint(-60, 1, (K,), device="cuda").float())
+    got = ops.tape8_linear_bwd(dz, t, w, act)
+    check_own(dz, t, w, act, got)
+    loud = w.clone()
+    loud[:, ::5] *= 2.0 ** 40
+    rest = torch.arange(K, device="cuda") % 5 != 0
+    assert torch.equal(ops.tape8_linear_bwd(dz, t, loud, act)[0][:, rest], got[0][:, rest])
 
 
 @pytest.mark.parametrize("act", ["relu", "none"])
