@@ -14,7 +14,7 @@
 // All four sums over rows are linear in  S1 = sum gate D f^,  S0 = sum gate D,  P1 = sum gh y^,  P0 = sum gh  - four sums per column.
 //
 // Both are bound by HBM: every array is read or written once.  Measured at 262 144 x 128 fp32 with a gate for each of four runs of rows:
-// with both tapes 122 us (5.0 TB/s), backward 117 + 9 us for the parameters' sums (4.7 TB/s); a large copy reaches 4.9.  A row belongs to a team of 16 to 512 lanes, four neighbouring columns per
+// with both tapes 116 - 130 us (from run to run; 4.9 TB/s in the middle), backward 111 - 120 + 9 us for the parameters' sums (4.7 TB/s); a large copy reaches 4.9.  A row belongs to a team of 16 to 512 lanes, four neighbouring columns per
 // lane and slot, at most two slots: it stays in registers from its load to its last use, and the next row of the team is loaded before this
 // one is worked on (the statistics are two dependent sums over the row: without rows in flight behind them the loads' latency is what
 // the kernel takes).  Sums over a team are lane exchanges inside the vector unit, through LDS for a team of several waves; fp32, the

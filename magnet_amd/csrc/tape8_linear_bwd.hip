@@ -2,10 +2,11 @@
 //     x  = act(v)   v = the tape's value: the activated input itself (none, relu) or Swish's argument (swish)
 //     dx [M][K] = act'(v) (dz W)        dW [N][K] (+)= dz^T x        db [N] (+)= column sums of dz
 // What has to move is dz in, dx out and 33/32 bytes a value of the tape: 1156 bytes a row at N = K = 128, where fp32 activations make it
-// 1536 (linear_bwd.hip).  Measured: 2 097 152 rows of 128 x 128 behind a ReLU 522 us (4.6 TB/s; a large copy reaches 4.9; the kernel
-// that reads fp32 activations 657 on the same box), 218 453 rows of 64 x 64 30 us, 262 144 rows of 128 x 128 behind Swish 105 us (20 of
-// them to start up and to add the partial sums; the exponentials, the second plane and the third product take turns with the loads: a
-// SIMD runs its vector and its matrix instructions at the sum of their times).
+// 1536 (linear_bwd.hip).  Measured, a call: 2 097 152 rows of 128 x 128 behind a ReLU 545 us (4.4 TB/s; a large copy reaches 4.9; the kernel
+// that reads fp32 activations 672 on the same box), 218 453 rows of 64 x 64 36.5 us (30 in this kernel), 262 144 rows of 128 x 128 behind Swish
+// 113 us.  Behind Swish 44 % of the SIMDs' cycles issue vector instructions and 22 % matrix ones, and a wave waits 45 % of its own: one
+// workgroup a CU, whose waves all form exponentials, meet and then all multiply.  (Where two variants are compared below, both were measured
+// with one scale for all rows of a workgroup: 3 % faster, 4 % behind Swish.)
 //
 // A workgroup of four or eight waves takes steps of 32 or 64 rows of one block of at most 128 x 128 of W.  dz is split once into two fp16 planes
 // (h + l, 22 bits), the tape's codes need one plane - a code has 8 bits, fp16 holds code times a power of two exactly - (two behind
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     // ---- the wave's features of W^T: A operands (lane = feature of x, register j of k group q4 = feature 32 t + 8 q4 + j of dz)
     t8_h8 wh[NBK][NT], wl[NBK][NT];
     unsigned we[NBK];                                                         // a feature of x is staged times 2^(140 - its exponent): max |W| over dz -> [2^13, 2^14);
-                                                                              // those of features 4 q4 .. + 3 of a block, a byte each (what the lane gets of dx)
+                                                                              // kept of features 4 q4 .. + 3 of a block, a byte each: what the lane gets of dx
     {
         auto w_at = [&](int b, int t, int j) -> float {
             const int n = 32 * t + 8 * q4 + j, k = k0 + kf + 16 * b + n16;
@@ -620,7 +621,7 @@ extern "C" int magnet_tape8_linear_bwd_f32(const float* dz, long ldz, const void
         a.M = M, a.ldz = ldz, a.ldw = ldw, a.lddx = lddx, a.N = n, a.K = K, a.ldc = (K + 31) / 32 * 32;
         a.exact = n == np && !(K % kp);
         a.add_dx = n0 > 0;
-        // (32-bit byte offsets inside a step of 32 rows)
+        // (32-bit byte offsets inside a lane's part of a step)
         const bool full = M >= 64 && N <= T8_BLOCK && !(n & 3) && !(K & 3) && ldz < (1l << 24) && lddx < (1l << 24) && ldw < (1l << 24);
         for (a.kb0 = 0; a.kb0 < kb; a.kb0 += T8_KBLOCKS) {
             const int kbn = kb - a.kb0 < T8_KBLOCKS ? kb - a.kb0 : T8_KBLOCKS;

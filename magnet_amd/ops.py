@@ -975,7 +975,11 @@ def tape8_linear_bwd(dz, tape: Tape8, w, act="none", *, need_dx=True, dx=None, d
     """A Linear (weight ``w`` [N, K]) walked back from the 8-bit tape of its input, in one pass over the rows: with v the tape's values and
     x = act(v), dx [M, K] = act'(v) (dz w), dW [N, K] (+)= dz^T x, db [N] (+)= column sums of dz -> (dx or None, dW, db).  ``act``: "none"
     (signed tape of x), "relu" (relu tape of x), "swish" (signed tape of Swish's argument).  fp32; ``accumulate`` adds to the dW and db
-    that are handed in."""
+    that are handed in.
+
+    dz and w enter as 22 bits of every value (two fp16 pieces), at a scale of each row of dz and each column of w: what lies 2^-39 under the row's,
+    2^-38 under the column's (in 128 rows of w) largest value is lost.  In dW rows whose product of largest gradient and largest value of a
+    block of 32 columns lies 2^-25 and more under the greatest such product that their workgroup has met lose what is under 2^-32 of it."""
     if act not in _T8_ACTS:
         raise ValueError(f"magnet_amd: act {act!r}; supported: {', '.join(_T8_ACTS)}")
     w = _matrix(w, "w", (torch.float32,))
