@@ -252,32 +252,23 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
     // ---- the exponents of this lane's rows of dz and, the last one, of the row that its codes belong to.  0: a row of zeros (what is not finite does not
     // count); 14 at least otherwise, so that 2^(141 - e) is a number
     auto measure = [&](int (&e)[NLD + 1]) {
-        auto rows = [&](bool finite) -> unsigned {
-            unsigned m[NLD];
+        // a magnitude's bits with the exponent one up in the top byte: what is not finite wraps to under the zero's 2^24
+        unsigned m[NLD];
 #pragma unroll
-            for (int i = 0; i < NLD; ++i) {
-                m[i] = 0u;
+        for (int i = 0; i < NLD; ++i) {
+            m[i] = 0u;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const unsigned b = __float_as_uint(dv[i][c]) & 0x7FFFFFFFu;
-                    m[i] = max(m[i], finite && b >= 0x7F800000u ? 0u : b);
-                }
-            }
-            return t8_row_max<NLD, LPR>(m, lane);
-        };
-        unsigned m = rows(false);
-        if (__any(m >= 0x7F800000u)) m = rows(true);
-        m = m == 0u ? 0u : max(m >> 23, 14u);
-        e[0] = (int)t8_dpp<0x00>(m), e[1] = (int)t8_dpp<0x55>(m);             // quad_perm 0 0 0 0, 1 1 1 1
-        if (NLD == 4) e[NLD - 2] = (int)t8_dpp<0xAA>(m), e[NLD - 1] = (int)t8_dpp<0xFF>(m);
+            for (int c = 0; c < 4; ++c) m[i] = max(m[i], (__float_as_uint(dv[i][c]) << 1) + (1u << 24));
+        }
+        const unsigned t = t8_row_max<NLD, LPR>(m, lane), x = t <= 1u << 24 ? 0u : max((t >> 24) - 1u, 14u);
+        e[0] = (int)t8_dpp<0x00>(x), e[1] = (int)t8_dpp<0x55>(x);             // quad_perm 0 0 0 0, 1 1 1 1
+        if (NLD == 4) e[NLD - 2] = (int)t8_dpp<0xAA>(x), e[NLD - 1] = (int)t8_dpp<0xFF>(x);
         const int p = lane / CPR % NLD;
         e[NLD] = p & 1 ? e[1] : e[0];
         if (NLD == 4) e[NLD] = p & 2 ? (p & 1 ? e[NLD - 1] : e[NLD - 2]) : e[NLD];
     };
-    // ---- this lane's part of the step in its two images, under the bounds; of Swish: the values and derivatives
-    typedef t8_f4 Vals[ACT == ACT_SWISH ? CW : 1];
-    auto stage = [&](Step& B, const int (&e)[NLD + 1], const Vals& y, const Vals& dy) {
-        const int ec = e[NLD];
+    // ---- this lane's part of the step in its two images: of dz ..
+    auto stage_z = [&](Step& B, const int (&e)[NLD + 1]) {
 #pragma unroll
         for (int i = 0; i < NLD; ++i) {
             const float G = FULL && zc >= a.N ? 0.f : __uint_as_float((unsigned)(268 - e[i]) << 23);         // 2^(141 - e); of zeros: some number
@@ -290,7 +281,11 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
             *reinterpret_cast<t8_u2*>(&B.z[0][zr + i][zc]) = h;
             *reinterpret_cast<t8_u2*>(&B.z[1][zr + i][zc]) = l;
         }
-        if (cc == 0) B.e[cr] = ec;
+        if (cc == 0) B.e[cr] = e[NLD];
+    };
+    // ---- .. and of x, under the bounds (ec: the exponent of its row of dz; of Swish: the values and derivatives)
+    typedef t8_f4 Vals[ACT == ACT_SWISH ? CW : 1];
+    auto stage_x = [&](Step& B, int ec, const Vals& y, const Vals& dy) {
         unsigned p[XPL][2 * CW];
         if (ACT == ACT_SWISH) {
             const float up = ec ? t8_pow2(268 + ec - ce) : 0.f;               // (a row without a gradient: nothing of it counts)
@@ -360,6 +355,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                 int e[NLD + 1];
                 Vals y, dy;
                 measure(e);
+                stage_z(B, e);
                 // the exponent of the largest product of this lane's row of dz and its part of x (the values' own, or the tape's byte); 0: none
                 int c = bv == 0u || bv == 255u ? 0 : (int)bv;
                 if (ACT == ACT_SWISH) {
@@ -396,7 +392,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                     for (int j = 0; j < TB; ++j) tce[j] = __builtin_amdgcn_readfirstlane(bound(xf / 32 + j, tce[j]));
                     if (tid < 2) flag[tid] = 0u;                              // (everybody has read the flag that ended the last stretch)
                 }
-                stage(B, e, y, dy);
+                stage_x(B, e[NLD], y, dy);
                 if (!fresh && __any(c > ce) && lane == 0) flag[it & 1] = 1u;
                 wg_barrier();
                 if (!fresh && __builtin_amdgcn_readfirstlane((int)flag[it & 1])) {          // (the same for every wave)
