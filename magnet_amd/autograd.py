@@ -106,8 +106,9 @@ class tape8:
     """``with tape8():`` around the forward of a training step: the MLP chains built inside keep their tape in 8 bits (ops.Tape8) - every
     hidden activation as codes that carry the ReLU mask exactly, the normalised row in place of the LayerNorm's input - and their
     backward walks the hidden Linears back from it (ops.tape8_linear_bwd).  A quarter of the memory between forward and backward, and gradients of
-    the same function with activations rounded to a step of at most 2 / 255 of their block's largest value.  ``tape8(False)``: off inside.  Like
-    ``torch.no_grad`` it holds for the thread that enters it."""
+    the same function with activations rounded to a step of at most 2 / 255 of their block's largest value; dz and
+    the weight enter with 22 bits, whichever split the chain's packs have.  ``tape8(False)``: off inside.  Like ``torch.no_grad`` it holds for
+    the thread that enters it."""
 
     def __init__(self, on=True):
         self.on = bool(on)

@@ -2,11 +2,11 @@
 //     x  = act(v)   v = the tape's value: the activated input itself (none, relu) or Swish's argument (swish)
 //     dx [M][K] = act'(v) (dz W)        dW [N][K] (+)= dz^T x        db [N] (+)= column sums of dz
 // What has to move is dz in, dx out and 33/32 bytes a value of the tape: 1156 bytes a row at N = K = 128, where fp32 activations make it
-// 1536 (linear_bwd.hip).  Measured, a call: 2 097 152 rows of 128 x 128 behind a ReLU 545 us (4.4 TB/s; a large copy reaches 4.9; the kernel
-// that reads fp32 activations 672 on the same box), 218 453 rows of 64 x 64 36.5 us (30 in this kernel), 262 144 rows of 128 x 128 behind Swish
-// 113 us.  Behind Swish 44 % of the SIMDs' cycles issue vector instructions and 22 % matrix ones, and a wave waits 45 % of its own: one
+// 1536 (linear_bwd.hip).  Measured, a call: 2 097 152 rows of 128 x 128 behind a ReLU 547 us (4.4 TB/s; a large copy reaches 4.9; the kernel
+// that reads fp32 activations 650 - 672), 218 453 rows of 64 x 64 37 us (30 - 32 in this kernel), 262 144 rows of 128 x 128 behind Swish
+// 112 us.  Behind Swish 44 % of the SIMDs' cycles issue vector instructions and 22 % matrix ones, and a wave waits 44 % of its own: one
 // workgroup a CU, whose waves all form exponentials, meet and then all multiply.  (Where two variants are compared below, both were measured
-// with one scale for all rows of a workgroup: 3 % faster, 4 % behind Swish.)
+// with one scale for all rows of a workgroup: 3 % faster.)
 //
 // A workgroup of four or eight waves takes steps of 32 or 64 rows of one block of at most 128 x 128 of W.  dz is split once into two fp16 planes
 // (h + l, 22 bits), the tape's codes need one plane - a code has 8 bits, fp16 holds code times a power of two exactly - (two behind
@@ -400,8 +400,7 @@ __global__ void __launch_bounds__(T8_WAVES(NP, KP) * 64, 2) k_tape8_linear_bwd(c
                     break;
                 }
 #pragma unroll
-                for (int i = 0; i < NLD; ++i)
-                    bsum += dv[i];
+                for (int i = 0; i < NLD; ++i) bsum += dv[i];
                 const long row0 = FULL ? min(step * R, a.M - R) : step * R;
                 const int done = shift;
                 asm volatile("" ::: "memory");
